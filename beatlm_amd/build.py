@@ -43,6 +43,10 @@ SOURCES = [
     "k_flash.hip",
     "k_misc.hip",
     "static_attention.hip",
+    "k_norm.hip",
+    "k_rotary.hip",
+    "k_packed.hip",
+    "ops.cpp",
     "backend.cpp",
     "timer.cpp",
     "ring.cpp",

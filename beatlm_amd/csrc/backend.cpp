@@ -25,6 +25,7 @@ using namespace bl;
 struct bl_ctx {
     int device = 0;
     hipStream_t stream = nullptr;
+    bool owns_stream = true;  // bl_ctx_create's; bl_ctx_create_on's is the host's
     std::string error;
     uint64_t allocations = 0;
     uint64_t device_bytes = 0;  // held now by the context's arenas and kernels
@@ -99,7 +100,7 @@ static void kernels_written(bl_kernels *k, uint32_t arena, uint64_t offset, uint
 
 extern "C" uint32_t bl_abi_version(void) { return BL_ABI_VERSION; }
 
-extern "C" int bl_ctx_create(int device_ordinal, bl_ctx **out) {
+static int ctx_create(int device_ordinal, bool owns_stream, hipStream_t stream, bl_ctx **out) {
     if (!out) return BL_ERR_INVALID_ARGUMENT;
     *out = nullptr;
     int count = 0;
@@ -115,7 +116,9 @@ extern "C" int bl_ctx_create(int device_ordinal, bl_ctx **out) {
     hipDeviceProp_t prop;
     if ((e = hipGetDeviceProperties(&prop, device_ordinal)) != hipSuccess) { delete ctx; return BL_ERR_HIP; }
     // One stream at the default priority; the frame loop's work is ordered on it.
-    if ((e = hipStreamCreateWithFlags(&ctx->stream, hipStreamNonBlocking)) != hipSuccess) {
+    ctx->owns_stream = owns_stream;
+    ctx->stream = stream;
+    if (owns_stream && (e = hipStreamCreateWithFlags(&ctx->stream, hipStreamNonBlocking)) != hipSuccess) {
         delete ctx;
         return BL_ERR_HIP;
     }
@@ -149,9 +152,24 @@ extern "C" int bl_ctx_create(int device_ordinal, bl_ctx **out) {
     return BL_OK;
 }
 
+extern "C" int bl_ctx_create(int device_ordinal, bl_ctx **out) {
+    return ctx_create(device_ordinal, true, nullptr, out);
+}
+
+extern "C" int bl_ctx_create_on(int device_ordinal, void *stream, bl_ctx **out) {
+    if (!out) return BL_ERR_INVALID_ARGUMENT;
+    *out = nullptr;
+    if (stream) {
+        hipDevice_t device = -1;
+        if (hipStreamGetDevice((hipStream_t)stream, &device) != hipSuccess) return BL_ERR_INVALID_ARGUMENT;
+        if (device != device_ordinal) return BL_ERR_INVALID_ARGUMENT;
+    }
+    return ctx_create(device_ordinal, false, (hipStream_t)stream, out);
+}
+
 static void ctx_free(bl_ctx *ctx) {
     hipSetDevice(ctx->device);
-    if (ctx->stream) {
+    if (ctx->owns_stream && ctx->stream) {
         hipStreamSynchronize(ctx->stream);
         hipStreamDestroy(ctx->stream);
     }
@@ -2246,6 +2264,7 @@ extern "C" int bl_kernels_create_internal(bl_ctx *ctx, bl_arenas *arenas, const 
         apply_folds(ks);
     }
     if (getenv("BL_NO_GRAPH") || profiler_attached()) ks->graphs_ok = false;
+    if (!ctx->owns_stream) ks->graphs_ok = false;  // the host may be capturing its stream itself
     bl_ctx_retain(ctx);
     arenas->users.push_back(ks);
     *out = ks;

@@ -17,3 +17,17 @@ uint32_t bl_compute_units_of(const bl_ctx *ctx);
 uint32_t bl_f32_math_of(const bl_ctx *ctx);
 // Sets the context's message (no allocation for messages under 512 bytes).
 int bl_fail(bl_ctx *ctx, int code, const char *msg);
+
+// Makes `device` current for a call and restores the caller's device after.
+struct DeviceScope {
+    int prev = -1;
+    hipError_t status = hipSuccess;
+    explicit DeviceScope(int device) {
+        status = hipGetDevice(&prev);
+        if (status == hipSuccess && prev != device) status = hipSetDevice(device);
+        else if (status == hipSuccess) prev = -1;  // already current: nothing to restore
+    }
+    ~DeviceScope() {
+        if (prev >= 0) hipSetDevice(prev);
+    }
+};

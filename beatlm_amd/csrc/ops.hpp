@@ -1,0 +1,57 @@
+// The packed attention sublayer's operators (include/beatlm_ops.h): what the
+// host side (ops.cpp) hands to the kernels (k_norm.hip, k_rotary.hip,
+// k_packed.hip). Every launch function checks nothing: ops.cpp has.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "../../include/beatlm_ops.h"
+
+namespace bl {
+
+// ---- LayerNorm ----
+
+struct NormParams {
+    const void *x, *gamma, *beta, *dy;
+    void *y, *dx;
+    float *mean, *rstd, *d_gamma, *d_beta;
+    float *partial;  // [groups][2][cols]: d_gamma's and d_beta's sums of one workgroup's rows
+    uint64_t x_stride, y_stride, dy_stride, dx_stride;
+    uint32_t rows, cols, groups;
+    float epsilon;
+    bool vector;  // every row of every tensor starts at 16 bytes and holds whole 16-byte chunks
+};
+// Workgroups of the backward: what its workspace holds a partial sum of each for.
+uint32_t norm_groups(uint32_t rows, uint32_t cols, uint32_t compute_units);
+hipError_t launch_norm_forward(const NormParams &p, uint32_t dtype, hipStream_t s);
+hipError_t launch_norm_backward(const NormParams &p, uint32_t dtype, hipStream_t s);
+
+// ---- rotary positions ----
+
+struct RotaryParams {
+    bl_rotary_table table;
+    const int32_t *positions;
+    bl_heads q_in, q_out, k_in, k_out;
+    uint32_t rows, q_heads, k_heads, head_dim;
+    float sign;       // -1: the inverse
+    bool copy_q, copy_k;  // channels beyond the pairs are copied (not when in place)
+    bool vector;
+};
+hipError_t launch_rotary(const RotaryParams &p, uint32_t dtype, uint32_t compute_units, hipStream_t s);
+
+// ---- attention over packed documents ----
+
+struct PackedParams {
+    bl_packed_attention_args a;
+    bl_packed_attention_grads g;
+    float *delta;    // [q_heads][q_rows]: sum_j P_ij dP_ij of each row
+    float *d_slope;  // [q_heads][q_rows]: each row's part of d_slopes, or null
+};
+struct PackedPlan {
+    uint64_t forward_bytes, backward_bytes;
+};
+PackedPlan plan_packed(const bl_packed_attention_args &a, uint32_t compute_units);
+hipError_t launch_packed_forward(const PackedParams &p, const PackedPlan &plan, hipStream_t s);
+hipError_t launch_packed_backward(const PackedParams &p, const PackedPlan &plan, hipStream_t s);
+
+}  // namespace bl

@@ -56,20 +56,6 @@ hipError_t scratch_on(int device, void **out) {
     return hipSuccess;
 }
 
-// Makes `device` current for the call and restores the caller's device after.
-struct DeviceScope {
-    int prev = -1;
-    hipError_t status = hipSuccess;
-    explicit DeviceScope(int device) {
-        status = hipGetDevice(&prev);
-        if (status == hipSuccess && prev != device) status = hipSetDevice(device);
-        else if (status == hipSuccess) prev = -1;  // already current: nothing to restore
-    }
-    ~DeviceScope() {
-        if (prev >= 0) hipSetDevice(prev);
-    }
-};
-
 int fail(bl_ctx *ctx, int code, const char *fmt, unsigned long long a, unsigned long long b) {
     char msg[256];
     snprintf(msg, sizeof msg, fmt, a, b);

@@ -167,6 +167,7 @@ _VP = C.c_void_p
 _SIGNATURES = {
     "bl_abi_version": (C.c_uint32, []),
     "bl_ctx_create": (C.c_int, [C.c_int, C.POINTER(_VP)]),
+    "bl_ctx_create_on": (C.c_int, [C.c_int, _VP, C.POINTER(_VP)]),
     "bl_ctx_destroy": (None, [_VP]),
     "bl_last_error": (C.c_char_p, [_VP]),
     "bl_device_profile": (C.c_int, [_VP, C.POINTER(DeviceProfile)]),
@@ -248,14 +249,21 @@ class BackendError(RuntimeError):
 
 
 class Context:
-    """One device, one stream (bl_ctx)."""
+    """One device, one stream (bl_ctx): a stream of its own, or with `stream`
+    the host's (a hipStream_t as an integer, 0 the device's default stream),
+    which the host keeps alive."""
 
-    def __init__(self, device: int = 0):
+    handle = None
+
+    def __init__(self, device: int = 0, stream: int | None = None):
         self._lib = lib()
         h = C.c_void_p()
-        rc = self._lib.bl_ctx_create(device, C.byref(h))
+        if stream is None:
+            rc = self._lib.bl_ctx_create(device, C.byref(h))
+        else:
+            rc = self._lib.bl_ctx_create_on(device, stream, C.byref(h))
         if rc != OK:
-            raise BackendError(rc, f"bl_ctx_create({device}) failed")
+            raise BackendError(rc, f"no context on device {device}" if stream is None else f"no context on device {device} over stream {stream:#x}")
         self.handle = h
 
     def check(self, rc: int) -> int:
