@@ -45,7 +45,10 @@ SOURCES = [
     "static_attention.hip",
     "k_norm.hip",
     "k_rotary.hip",
-    "k_packed.hip",
+    "k_packed_f32.hip",
+    "k_packed_f16.hip",
+    "k_packed_bf16.hip",
+    "packed_plan.cpp",
     "ops.cpp",
     "backend.cpp",
     "timer.cpp",

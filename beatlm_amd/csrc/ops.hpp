@@ -44,14 +44,27 @@ hipError_t launch_rotary(const RotaryParams &p, uint32_t dtype, uint32_t compute
 struct PackedParams {
     bl_packed_attention_args a;
     bl_packed_attention_grads g;
-    float *delta;    // [q_heads][q_rows]: sum_j P_ij dP_ij of each row
-    float *d_slope;  // [q_heads][q_rows]: each row's part of d_slopes, or null
+    // forward, when keys are split: each split's sums, unscaled, and their (maximum, total)
+    uint32_t splits;
+    float *partial;  // [splits][q_rows * q_heads][tile_dim]
+    float *stats;    // [splits][q_rows * q_heads][2]
+    // backward, [q_heads][q_rows] each
+    float *delta;    // sum_c dO O of each row
+    float *largest;  // its largest |dO| (f16)
+    float *d_slope;  // its part of d_slopes, or null
 };
 struct PackedPlan {
+    uint32_t splits;
+    uint32_t tile_dim;  // channels of the kernels' tiles: 64 or 128
+    uint64_t partial_bytes, stats_bytes, row_bytes;
     uint64_t forward_bytes, backward_bytes;
 };
 PackedPlan plan_packed(const bl_packed_attention_args &a, uint32_t compute_units);
 hipError_t launch_packed_forward(const PackedParams &p, const PackedPlan &plan, hipStream_t s);
 hipError_t launch_packed_backward(const PackedParams &p, const PackedPlan &plan, hipStream_t s);
+
+// One element type each (k_packed_*.hip).
+template <typename T> hipError_t packed_forward(const PackedParams &p, const PackedPlan &plan, hipStream_t s);
+template <typename T> hipError_t packed_backward(const PackedParams &p, const PackedPlan &plan, hipStream_t s);
 
 }  // namespace bl

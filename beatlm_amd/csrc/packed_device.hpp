@@ -1,11 +1,17 @@
 // What the packed attention kernels share: a document's bounds, clamped to
-// the tensors whatever the offset arrays hold, and the score of a (query,
-// key) pair.
+// the tensors whatever the offset arrays hold; which document and tile a
+// workgroup has; matrix core operands of the three element types; tiles of
+// rows staged through LDS; scores.
 #pragma once
 
 #include "ops_device.hpp"
 
 namespace bl {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+
+// ---- documents ----
 
 struct Document {
     int q0, n_q;     // first query row, query rows
@@ -28,30 +34,242 @@ __device__ __forceinline__ Document document_of(const bl_packed_attention_args &
     return doc;
 }
 
-// The document that holds row `row` by `offsets` (documents + 1 of them, or
-// null: one), or -1.
-__device__ __forceinline__ int document_at(const int32_t *offsets, uint32_t documents, int row) {
-    if (!offsets) return 0;
-    int lo = 0, hi = (int)documents;  // the first offset beyond row lies in (lo, hi]
-    if (row < offsets[0] || row >= offsets[documents]) return -1;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (offsets[mid] <= row) lo = mid;
-        else hi = mid;
+// Keys [0, limit) of the document are what its query i sees.
+__device__ __forceinline__ int limit_of(const bl_packed_attention_args &a, const Document &doc, int i) {
+    return a.mask == BL_MASK_NONE ? doc.n_k : min(doc.n_k, max(i + doc.shift + 1, doc.prefix));
+}
+
+// The tiles of all documents have one grid: document d's tiles of `tile`
+// places (its rows times `times`) start at slot first * times / tile + d,
+// which leaves room for each document's last, partial tile whatever the
+// lengths are. slots() is the grid; document_of_slot finds the document whose
+// first slot is the last one not beyond `slot` (64 candidates a step, one
+// load), or 0.
+__host__ __device__ __forceinline__ uint32_t slots(uint32_t rows, uint32_t times, uint32_t tile, uint32_t documents) {
+    return (uint32_t)((uint64_t)rows * times / tile) + documents;
+}
+__device__ __forceinline__ int first_slot(const int32_t *offsets, int d, int rows, int times, int tile) {
+    return (int)((int64_t)min(max(offsets[d], 0), rows) * times / tile) + d;
+}
+__device__ __forceinline__ int document_of_slot(const int32_t *offsets, int documents, int rows, int times, int tile, int slot) {
+    if (!offsets || documents == 1) return 0;
+    const int lane = threadIdx.x % 64;
+    int lo = 0, count = documents;  // the answer is in [lo, lo + count)
+    while (count > 1) {
+        const int step = (count + 63) / 64;
+        const int d = lo + lane * step;
+        const bool before = lane * step < count && first_slot(offsets, d, rows, times, tile) <= slot;
+        const int last = __popcll(__ballot(before)) - 1;  // first slots rise with d
+        const int at = max(last, 0) * step;
+        lo += at;
+        count = min(step, count - at);
     }
-    return lo;
+    return __builtin_amdgcn_readfirstlane(lo);
 }
 
-__device__ __forceinline__ bool visible(const bl_packed_attention_args &a, const Document &doc, int i, int j) {
-    return a.mask == BL_MASK_NONE || j <= i + doc.shift || j < doc.prefix;
+// ---- matrix core operands ----
+//
+// Every product here runs on 32 x 32 tiles: C[row][col] is held by lane
+// (half h = lane / 32, col = lane % 32), register r at row
+// 8 (r / 4) + 4 h + r % 4. An operand is a 16-byte chunk a lane: KS / 2
+// elements of the contraction for its row (A) or column (B), the two halves
+// sharing a step of KS. Which of the step's elements a half holds is free as
+// long as A and B agree:
+//  - for operands read along their rows, half h has elements KS/2 h + [0, KS/2);
+//  - for a product over a tile's rows or columns just computed (probabilities),
+//    half h has those its registers hold: 8 (j / 4) + 4 h + j % 4 of 16 for the
+//    16-bit types, 4 h + j of 8 for f32. The other operand is read transposed
+//    in the same order, so no value changes lanes.
+
+template <typename T> struct Mma;
+template <> struct Mma<_Float16> {
+    typedef f16x8 Frag;
+    static constexpr int KS = 16;
+    static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct Mma<__bf16> {
+    typedef bf16x8 Frag;
+    static constexpr int KS = 16;
+    static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct Mma<float> {
+    typedef f32x4 Frag;
+    static constexpr int KS = 8;
+    static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+        return c;
+    }
+};
+
+// KS values of a tile's registers (16-bit: registers 8 t .. 8 t + 7, f32:
+// 4 t .. 4 t + 3) as an operand of step t: the one rounding of probabilities
+// and scores' gradients to the tensors' type, which the matrix cores ask for.
+template <typename T>
+__device__ __forceinline__ typename Mma<T>::Frag operand_of(const f32x16 &v, int t) {
+    typename Mma<T>::Frag f;
+    constexpr int N = Mma<T>::KS / 2;
+#pragma unroll
+    for (int j = 0; j < N; j++) f[j] = (T)v[N * t + j];
+    return f;
 }
 
-__device__ __forceinline__ float distance_of(const bl_packed_attention_args &a, const Document &doc, int i, int j) {
-    if (!a.axes) return (float)abs(i + doc.shift - j);
-    int sum = 0;
-    for (uint32_t x = 0; x < a.axes; x++)
-        sum += abs(a.q_positions[(int64_t)(doc.q0 + i) * a.axes + x] - a.k_positions[(int64_t)(doc.k0 + j) * a.axes + x]);
-    return (float)sum;
+// ---- tiles of rows in LDS ----
+//
+// ROWS rows of D channels, 16-byte chunks, brought by buffer loads straight
+// into LDS. The buffer ends with the last row the document owns and a lane
+// beyond head_dim points outside, and what lies outside arrives as zeros: no
+// row of another document is read, and no padding is left to chance. Chunks
+// lie in LDS in the loads' order, which is linear in the lane, so a row's
+// chunks are permuted on the global side: position x holds chunk
+// x ^ swizzle(row), which spreads both the reads along rows (16 rows, one
+// chunk each) and the transposed ones (8 rows, 4 neighbouring chunks each)
+// over all 64 banks.
+
+template <typename T, int D, int ROWS> struct Tile {
+    typedef typename Mma<T>::Frag Frag;
+    static constexpr int CHUNKS = D * (int)sizeof(T) / 16;  // of a row: 8, 16 or 32
+    static constexpr int ROW = D * (int)sizeof(T);
+    static constexpr int BYTES = ROWS * ROW;
+    static constexpr int LOADS = ROWS * CHUNKS / 256;        // a thread's, of 256 threads
+    static constexpr int STEPS = D / Mma<T>::KS;             // of a product over channels
+
+    static __device__ __forceinline__ int swizzle(int row) {
+        if constexpr (CHUNKS == 8) return ((row & 2) << 1) | ((row >> 2) & 3);
+        else if constexpr (sizeof(T) == 2) return ((row & 3) << 2) | ((row >> 2) & 3);
+        else return (row & 3) | ((row & 4) << 1) | ((row & 8) >> 1);
+    }
+
+    // Byte offsets of this thread's chunks from the tile's first row.
+    uint32_t offset[LOADS];
+    uint32_t stride, end;  // bytes from a row to the next; of the last row
+
+    __device__ __forceinline__ Tile(uint64_t row_stride, uint32_t head_dim) {
+        stride = (uint32_t)row_stride * sizeof(T);
+        end = head_dim * sizeof(T);
+#pragma unroll
+        for (int n = 0; n < LOADS; n++) {
+            const int i = n * 256 + threadIdx.x;
+            const int row = i / CHUNKS, chunk = (i % CHUNKS) ^ swizzle(row);
+            offset[n] = chunk * 16 < (int)end ? (uint32_t)row * stride + chunk * 16 : 0x7ffffff0u;
+        }
+    }
+    // Starts the loads of up to `left` rows (at least one) from `base` into `lds`.
+    __device__ __forceinline__ void load(const char *base, int left, char *lds) const {
+#ifdef __HIP_DEVICE_COMPILE__  // the host pass knows no 16-byte loads to LDS
+        const uint32_t records = (uint32_t)(min(left, ROWS) - 1) * stride + end;
+        const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, records, 0x00020000);
+        const int wave = threadIdx.x / 64;
+#pragma unroll
+        for (int n = 0; n < LOADS; n++)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void *)(lds + (n * 256 + wave * 64) * 16), 16,
+                                                     offset[n], 0, 0, 0);
+#endif
+    }
+    // The operand of row `row` (the lane's) and step t along the channels.
+    static __device__ __forceinline__ Frag along(const char *lds, int row, int half, int t) {
+        return *(const Frag *)(lds + row * ROW + (((2 * t + half) ^ swizzle(row)) * 16));
+    }
+    // The transposed operand: channel 32 block + lane % 32, rows of step t.
+    static __device__ __forceinline__ Frag across(const char *lds, int lane, int t, int block) {
+        const int half = lane / 32;
+        if constexpr (sizeof(T) == 2) {
+            // 16 lanes bring a 4 x 16 piece: lane i row i / 4, channels 4 (i % 4) ..; each gets its column.
+            const int i = lane % 16, chunk = 4 * block + 2 * ((lane / 16) % 2) + (i % 4) / 2;
+            const int row = 16 * t + 4 * half + i / 4;
+            typedef short s16x4 __attribute__((ext_vector_type(4)));
+            const auto at = [&](int r) {
+                return (__attribute__((address_space(3))) s16x4 *)(lds + r * ROW + (chunk ^ swizzle(r)) * 16 + (i % 2) * 8);
+            };
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at(row));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at(row + 8));
+            return __builtin_bit_cast(Frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        } else {
+            const int c = 32 * block + lane % 32;
+            Frag f;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int row = 8 * t + 4 * half + j;
+                f[j] = *(const float *)(lds + row * ROW + ((c / 4) ^ swizzle(row)) * 16 + (c % 4) * 4);
+            }
+            return f;
+        }
+    }
+    static __device__ __forceinline__ T *element(char *lds, int row, int c) {
+        constexpr int PER = 16 / sizeof(T);
+        return (T *)(lds + row * ROW + ((c / PER) ^ swizzle(row)) * 16) + c % PER;
+    }
+};
+
+// A lane's row of a tensor as operands along the channels, zeros beyond
+// head_dim and for no row.
+template <typename T, int D>
+__device__ __forceinline__ void load_row(const bl_heads &h, bool there, int64_t row, int64_t head, int half, uint32_t head_dim,
+                                         typename Mma<T>::Frag (&f)[D / Mma<T>::KS]) {
+    typedef typename Mma<T>::Frag Frag;
+    constexpr int KS = Mma<T>::KS;
+    const T *at = (const T *)h.data + row * (int64_t)h.row_stride + head * (int64_t)h.head_stride;
+#pragma unroll
+    for (int t = 0; t < D / KS; t++) {
+        const uint32_t c = t * KS + half * (KS / 2);
+        f[t] = there && c < head_dim ? *(const Frag *)(at + c) : Frag{};
+    }
 }
+
+// An accumulator C[channel][the lane's row] of D / 32 blocks, times `by`, to
+// the lane's row of a tensor.
+template <typename T, int D>
+__device__ __forceinline__ void store_row(const bl_heads &h, int64_t row, int64_t head, int half, uint32_t head_dim, const f32x16 (&acc)[D / 32],
+                                          float by) {
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    T *at = (T *)h.data + row * (int64_t)h.row_stride + head * (int64_t)h.head_stride;
+#pragma unroll
+    for (int b = 0; b < D / 32; b++)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            const uint32_t c = 32 * b + 2 * r + 4 * half;
+            T4 v;
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = (T)(acc[b][r + e] * by);
+            if (c < head_dim) *(T4 *)(at + c) = v;  // head_dim is a multiple of 8
+        }
+}
+
+// ---- scores ----
+//
+// In base two: x = log2(e) s, so probabilities are exp2(x - .). With a cap,
+// s = cap tanh(u), u = scale qk / cap.
+
+struct ScoreConstants {
+    float scale2;    // log2(e) scale: x per qk, uncapped
+    float tanh2;     // 2 log2(e) scale / cap: the exponent of tanh's exponential per qk
+    float inner;     // scale / cap
+    float cap2;      // log2(e) cap
+    __device__ __forceinline__ explicit ScoreConstants(const bl_packed_attention_args &a) {
+        scale2 = a.scale * LOG2E;
+        inner = a.softcap > 0.0f ? a.scale / a.softcap : 0.0f;
+        tanh2 = 2.0f * LOG2E * inner;
+        cap2 = a.softcap * LOG2E;
+    }
+};
+
+// x of one product, and with a cap its tanh. The 16-bit types take
+// tanh u = 1 - 2 / (e^2u + 1), good to a few steps of 1 (their own steps are
+// 2^13 and 2^16 times that); f32 takes tanhf, good to steps of the result.
+template <typename T, bool CAP>
+__device__ __forceinline__ float score(const ScoreConstants &k, float qk, float &th) {
+    if constexpr (!CAP) {
+        return qk * k.scale2;
+    } else if constexpr (sizeof(T) == 4) {
+        th = tanhf(qk * k.inner);
+        return th * k.cap2;
+    } else {
+        th = 1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(qk * k.tanh2) + 1.0f);
+        return th * k.cap2;
+    }
+}
+
+// Sum over axes of |a - b|, axes beyond `axes` left out.
+__device__ __forceinline__ uint32_t apart(int a, int b) { return a > b ? (uint32_t)a - (uint32_t)b : (uint32_t)b - (uint32_t)a; }
 
 }  // namespace bl

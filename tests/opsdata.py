@@ -188,12 +188,20 @@ class Packed:
                 # 1 - tanh^2 is off by a few steps of 1 and by twice the score's error over the cap
                 inner_off = abs(self.scale) * (ds_off * slack + ds.abs() * (16 * F32 + (4 * off / self.cap if self.cap else 0.0)))
                 inner_off = inner_off + inner * inner_s.abs()
+                tiny = 0.0
+                if self.torch_dtype == torch.float16:
+                    # Operands below f16's smallest normal number, 2^-14, are off by half its
+                    # smallest step, 2^-25: P itself, and dS divided by a power of two that is
+                    # at most the largest |dO| of the key head's rows.
+                    tiny = 2.0**-25
+                    heads = self.d_out[:, kv * group:(kv + 1) * group].double().nan_to_num(0.0)
+                    inner_off = inner_off + abs(self.scale) * tiny * heads.abs().max() * seen
                 d_q[0][rows, h] = inner_s @ k
                 d_q[1][rows, h] = u * d_q[0][rows, h].abs() + (inner_off + F32 * (n_k + 8) * inner_s.abs()) @ k.abs() + 1e-30
                 d_k[0][keys, kv] += inner_s.T @ q
                 d_k[1][keys, kv] += (inner_off + F32 * (group * n_q + 8) * inner_s.abs()).T @ q.abs()
                 d_v[0][keys, kv] += p.T @ g
-                d_v[1][keys, kv] += (p * (relative + inner + F32 * (group * n_q + 8))).T @ g.abs()
+                d_v[1][keys, kv] += (p * (relative + inner + F32 * (group * n_q + 8)) + tiny * seen).T @ g.abs()
                 if self.slopes is not None:
                     d_slopes[0][h] -= (ds * far).sum()
                     # through the row's own sums in f32: sum P dP far - (sum P dP)(sum P far)
