@@ -13,6 +13,10 @@ constexpr float LN2 = 0.6931471805599453f;
 
 // ---- documents ----
 
+// What every lane holds alike, in a scalar register: buffer descriptors and
+// branches want it there, and the compiler cannot always tell.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
 struct Document {
     int q0, n_q;     // first query row, query rows
     int k0, n_k;     // first key row, key rows
@@ -23,14 +27,14 @@ struct Document {
 __device__ __forceinline__ Document document_of(const bl_packed_attention_args &a, int d) {
     Document doc;
     const int q_rows = (int)a.q_rows, k_rows = (int)a.k_rows;
-    doc.q0 = a.q_offsets ? min(max(a.q_offsets[d], 0), q_rows) : 0;
+    doc.q0 = uniform(a.q_offsets ? min(max(a.q_offsets[d], 0), q_rows) : 0);
     const int q1 = a.q_offsets ? min(max(a.q_offsets[d + 1], 0), q_rows) : q_rows;
-    doc.n_q = max(q1 - doc.q0, 0);
-    doc.k0 = a.k_begin ? min(max(a.k_begin[d], 0), k_rows) : 0;
+    doc.n_q = uniform(max(q1 - doc.q0, 0));
+    doc.k0 = uniform(a.k_begin ? min(max(a.k_begin[d], 0), k_rows) : 0);
     const int k1 = a.k_begin ? min(max(a.k_end[d], 0), k_rows) : k_rows;
-    doc.n_k = max(k1 - doc.k0, 0);
+    doc.n_k = uniform(max(k1 - doc.k0, 0));
     doc.shift = doc.n_k - doc.n_q;
-    doc.prefix = a.mask == BL_MASK_PREFIX ? max(a.prefix[d], 0) : 0;
+    doc.prefix = uniform(a.mask == BL_MASK_PREFIX ? max(a.prefix[d], 0) : 0);
     return doc;
 }
 
@@ -66,6 +70,10 @@ __device__ __forceinline__ int document_of_slot(const int32_t *offsets, int docu
     }
     return __builtin_amdgcn_readfirstlane(lo);
 }
+
+// Nothing is scheduled across this: it bounds how many operands are in
+// registers at once where the compiler would fetch all of a loop's first.
+__device__ __forceinline__ void phase() { __builtin_amdgcn_sched_barrier(0); }
 
 // ---- matrix core operands ----
 //
@@ -137,7 +145,7 @@ template <typename T, int D, int ROWS> struct Tile {
     static __device__ __forceinline__ int swizzle(int row) {
         if constexpr (CHUNKS == 8) return ((row & 2) << 1) | ((row >> 2) & 3);
         else if constexpr (sizeof(T) == 2) return ((row & 3) << 2) | ((row >> 2) & 3);
-        else return (row & 3) | ((row & 4) << 1) | ((row & 8) >> 1);
+        else return row & 7;
     }
 
     // Byte offsets of this thread's chunks from the tile's first row.
@@ -157,43 +165,15 @@ template <typename T, int D, int ROWS> struct Tile {
     // Starts the loads of up to `left` rows (at least one) from `base` into `lds`.
     __device__ __forceinline__ void load(const char *base, int left, char *lds) const {
 #ifdef __HIP_DEVICE_COMPILE__  // the host pass knows no 16-byte loads to LDS
-        const uint32_t records = (uint32_t)(min(left, ROWS) - 1) * stride + end;
-        const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, records, 0x00020000);
-        const int wave = threadIdx.x / 64;
+        const uint32_t records = uniform((min(left, ROWS) - 1) * (int)stride + (int)end);
+        const uint64_t from = (uint64_t)(uint32_t)uniform((int)((uint64_t)base >> 32)) << 32 | (uint32_t)uniform((int)(uint64_t)base);
+        const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)from, 0, records, 0x00020000);
+        const int wave = uniform(threadIdx.x / 64);
 #pragma unroll
         for (int n = 0; n < LOADS; n++)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void *)(lds + (n * 256 + wave * 64) * 16), 16,
                                                      offset[n], 0, 0, 0);
 #endif
-    }
-    // The operand of row `row` (the lane's) and step t along the channels.
-    static __device__ __forceinline__ Frag along(const char *lds, int row, int half, int t) {
-        return *(const Frag *)(lds + row * ROW + (((2 * t + half) ^ swizzle(row)) * 16));
-    }
-    // The transposed operand: channel 32 block + lane % 32, rows of step t.
-    static __device__ __forceinline__ Frag across(const char *lds, int lane, int t, int block) {
-        const int half = lane / 32;
-        if constexpr (sizeof(T) == 2) {
-            // 16 lanes bring a 4 x 16 piece: lane i row i / 4, channels 4 (i % 4) ..; each gets its column.
-            const int i = lane % 16, chunk = 4 * block + 2 * ((lane / 16) % 2) + (i % 4) / 2;
-            const int row = 16 * t + 4 * half + i / 4;
-            typedef short s16x4 __attribute__((ext_vector_type(4)));
-            const auto at = [&](int r) {
-                return (__attribute__((address_space(3))) s16x4 *)(lds + r * ROW + (chunk ^ swizzle(r)) * 16 + (i % 2) * 8);
-            };
-            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at(row));
-            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at(row + 8));
-            return __builtin_bit_cast(Frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-        } else {
-            const int c = 32 * block + lane % 32;
-            Frag f;
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int row = 8 * t + 4 * half + j;
-                f[j] = *(const float *)(lds + row * ROW + ((c / 4) ^ swizzle(row)) * 16 + (c % 4) * 4);
-            }
-            return f;
-        }
     }
     static __device__ __forceinline__ T *element(char *lds, int row, int c) {
         constexpr int PER = 16 / sizeof(T);
@@ -201,8 +181,56 @@ template <typename T, int D, int ROWS> struct Tile {
     }
 };
 
+// A lane's places in a tile, found once: all that is left for a read is a
+// constant (LDS instructions take it) and one of a few registers.
+template <typename T, int D, int ROWS> struct Reader {
+    typedef Tile<T, D, ROWS> S;
+    typedef typename Mma<T>::Frag Frag;
+    static constexpr bool F32 = sizeof(T) == 4;
+    static constexpr int STEPS = F32 ? 4 : S::STEPS;       // steps until the places along a row repeat, 128 bytes on
+    static constexpr int PIECES = F32 ? 4 : D / 32 * 2;
+    int a[STEPS], b[PIECES];
+
+    __device__ __forceinline__ explicit Reader(int lane) {
+        const int half = lane / 32, row = lane % 32;
+#pragma unroll
+        for (int t = 0; t < STEPS; t++) a[t] = row * S::ROW + ((2 * t + half) ^ S::swizzle(row)) * 16;
+#pragma unroll
+        for (int n = 0; n < PIECES; n++) {
+            if constexpr (F32) {
+                const int r = 4 * half + n;
+                b[n] = r * S::ROW + ((lane % 32 / 4) ^ S::swizzle(r)) * 16 + lane % 4 * 4;
+            } else {
+                // 16 lanes bring a 4 x 16 piece: lane i row i / 4, channels 4 (i % 4) ..; each gets its column.
+                const int i = lane % 16, chunk = 4 * (n / 2) + 2 * (lane / 16 % 2) + i % 4 / 2;
+                const int r = 4 * half + i / 4 + n % 2 * 8;
+                b[n] = r * S::ROW + (chunk ^ S::swizzle(r)) * 16 + i % 2 * 8;
+            }
+        }
+    }
+    // The operand of rows r0 + lane % 32 (r0 a multiple of 32) and step t along the channels.
+    __device__ __forceinline__ Frag along(const char *lds, int r0, int t) const {
+        return *(const Frag *)(lds + a[t % STEPS] + (r0 * S::ROW + t / STEPS * 128));
+    }
+    // The transposed operand: channel 32 block + lane % 32, rows of step t.
+    __device__ __forceinline__ Frag across(const char *lds, int t, int block) const {
+        if constexpr (F32) {
+            Frag f;
+#pragma unroll
+            for (int j = 0; j < 4; j++) f[j] = *(const float *)(lds + b[j] + (8 * t * S::ROW + block * 128));
+            return f;
+        } else {
+            typedef short s16x4 __attribute__((ext_vector_type(4)));
+            const auto piece = [&](int n) {
+                return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(lds + b[2 * block + n] + 16 * t * S::ROW));
+            };
+            return __builtin_bit_cast(Frag, __builtin_shufflevector(piece(0), piece(1), 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+    }
+};
+
 // A lane's row of a tensor as operands along the channels, zeros beyond
-// head_dim and for no row.
+// head_dim and where the lane has none (`row` is then any row there is).
 template <typename T, int D>
 __device__ __forceinline__ void load_row(const bl_heads &h, bool there, int64_t row, int64_t head, int half, uint32_t head_dim,
                                          typename Mma<T>::Frag (&f)[D / Mma<T>::KS]) {
@@ -212,7 +240,9 @@ __device__ __forceinline__ void load_row(const bl_heads &h, bool there, int64_t 
 #pragma unroll
     for (int t = 0; t < D / KS; t++) {
         const uint32_t c = t * KS + half * (KS / 2);
-        f[t] = there && c < head_dim ? *(const Frag *)(at + c) : Frag{};
+        const bool in = c < head_dim;
+        const Frag v = *(const Frag *)(at + (in ? c : 0));
+        f[t] = there && in ? v : Frag{};
     }
 }
 
