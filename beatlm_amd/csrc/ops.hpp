@@ -44,19 +44,21 @@ hipError_t launch_rotary(const RotaryParams &p, uint32_t dtype, uint32_t compute
 struct PackedParams {
     bl_packed_attention_args a;
     bl_packed_attention_grads g;
-    // forward, when keys are split: each split's sums, unscaled, and their (maximum, total)
-    uint32_t splits;
-    float *partial;  // [splits][q_rows * q_heads][tile_dim]
-    float *stats;    // [splits][q_rows * q_heads][2]
+    // Where the streamed side is split over workgroups, each split's sums,
+    // joined by a launch of its own.
+    uint32_t splits, splits_q, splits_kv;
+    float *partial;  // forward [splits][places][tile_dim]; d_q [splits][2][places][tile_dim]; d_k, d_v [splits][2][k_rows * kv_heads][tile_dim]
+    float *stats;    // forward [splits][places][2], d_q [splits][places][4]; places = q_rows * q_heads
     // backward, [q_heads][q_rows] each
-    float *delta;    // sum_c dO O of each row
+    float *delta;    // sum_j P_j dP_j of each row
     float *largest;  // its largest |dO| (f16)
-    float *d_slope;  // its part of d_slopes, or null
+    float *d_slope;  // its part of d_slopes
 };
 struct PackedPlan {
-    uint32_t splits;
+    uint32_t splits, splits_q, splits_kv;
     uint32_t tile_dim;  // channels of the kernels' tiles: 64 or 128
-    uint64_t partial_bytes, stats_bytes, row_bytes;
+    uint64_t partial_bytes, stats_bytes;                     // forward
+    uint64_t row_bytes, back_partial_bytes, back_stats_bytes; // backward
     uint64_t forward_bytes, backward_bytes;
 };
 PackedPlan plan_packed(const bl_packed_attention_args &a, uint32_t compute_units);

@@ -134,12 +134,12 @@ __device__ __forceinline__ typename Mma<T>::Frag operand_of(const f32x16 &v, int
 // chunk each) and the transposed ones (8 rows, 4 neighbouring chunks each)
 // over all 64 banks.
 
-template <typename T, int D, int ROWS> struct Tile {
+template <typename T, int D, int ROWS, int THREADS = 256> struct Tile {
     typedef typename Mma<T>::Frag Frag;
     static constexpr int CHUNKS = D * (int)sizeof(T) / 16;  // of a row: 8, 16 or 32
     static constexpr int ROW = D * (int)sizeof(T);
     static constexpr int BYTES = ROWS * ROW;
-    static constexpr int LOADS = ROWS * CHUNKS / 256;        // a thread's, of 256 threads
+    static constexpr int LOADS = ROWS * CHUNKS / THREADS;    // a thread's, of the workgroup's
     static constexpr int STEPS = D / Mma<T>::KS;             // of a product over channels
 
     static __device__ __forceinline__ int swizzle(int row) {
@@ -157,7 +157,7 @@ template <typename T, int D, int ROWS> struct Tile {
         end = head_dim * sizeof(T);
 #pragma unroll
         for (int n = 0; n < LOADS; n++) {
-            const int i = n * 256 + threadIdx.x;
+            const int i = n * THREADS + threadIdx.x;
             const int row = i / CHUNKS, chunk = (i % CHUNKS) ^ swizzle(row);
             offset[n] = chunk * 16 < (int)end ? (uint32_t)row * stride + chunk * 16 : 0x7ffffff0u;
         }
@@ -171,7 +171,7 @@ template <typename T, int D, int ROWS> struct Tile {
         const int wave = uniform(threadIdx.x / 64);
 #pragma unroll
         for (int n = 0; n < LOADS; n++)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void *)(lds + (n * 256 + wave * 64) * 16), 16,
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void *)(lds + (n * THREADS + wave * 64) * 16), 16,
                                                      offset[n], 0, 0, 0);
 #endif
     }
@@ -183,15 +183,16 @@ template <typename T, int D, int ROWS> struct Tile {
 
 // A lane's places in a tile, found once: all that is left for a read is a
 // constant (LDS instructions take it) and one of a few registers.
-template <typename T, int D, int ROWS> struct Reader {
+template <typename T, int D, int ROWS, int BLOCKS = D / 32> struct Reader {
     typedef Tile<T, D, ROWS> S;
     typedef typename Mma<T>::Frag Frag;
     static constexpr bool F32 = sizeof(T) == 4;
     static constexpr int STEPS = F32 ? 4 : S::STEPS;       // steps until the places along a row repeat, 128 bytes on
-    static constexpr int PIECES = F32 ? 4 : D / 32 * 2;
+    static constexpr int PIECES = F32 ? 4 : BLOCKS * 2;
     int a[STEPS], b[PIECES];
 
-    __device__ __forceinline__ explicit Reader(int lane) {
+    // `first`: the first of the BLOCKS blocks of 32 channels that are read transposed.
+    __device__ __forceinline__ explicit Reader(int lane, int first = 0) {
         const int half = lane / 32, row = lane % 32;
 #pragma unroll
         for (int t = 0; t < STEPS; t++) a[t] = row * S::ROW + ((2 * t + half) ^ S::swizzle(row)) * 16;
@@ -199,10 +200,10 @@ template <typename T, int D, int ROWS> struct Reader {
         for (int n = 0; n < PIECES; n++) {
             if constexpr (F32) {
                 const int r = 4 * half + n;
-                b[n] = r * S::ROW + ((lane % 32 / 4) ^ S::swizzle(r)) * 16 + lane % 4 * 4;
+                b[n] = r * S::ROW + ((lane % 32 / 4) ^ S::swizzle(r)) * 16 + lane % 4 * 4 + first * 128;
             } else {
                 // 16 lanes bring a 4 x 16 piece: lane i row i / 4, channels 4 (i % 4) ..; each gets its column.
-                const int i = lane % 16, chunk = 4 * (n / 2) + 2 * (lane / 16 % 2) + i % 4 / 2;
+                const int i = lane % 16, chunk = 4 * (first + n / 2) + 2 * (lane / 16 % 2) + i % 4 / 2;
                 const int r = 4 * half + i / 4 + n % 2 * 8;
                 b[n] = r * S::ROW + (chunk ^ S::swizzle(r)) * 16 + i % 2 * 8;
             }
@@ -212,7 +213,7 @@ template <typename T, int D, int ROWS> struct Reader {
     __device__ __forceinline__ Frag along(const char *lds, int r0, int t) const {
         return *(const Frag *)(lds + a[t % STEPS] + (r0 * S::ROW + t / STEPS * 128));
     }
-    // The transposed operand: channel 32 block + lane % 32, rows of step t.
+    // The transposed operand: channel 32 (first + block) + lane % 32, rows of step t.
     __device__ __forceinline__ Frag across(const char *lds, int t, int block) const {
         if constexpr (F32) {
             Frag f;
@@ -246,23 +247,32 @@ __device__ __forceinline__ void load_row(const bl_heads &h, bool there, int64_t 
     }
 }
 
-// An accumulator C[channel][the lane's row] of D / 32 blocks, times `by`, to
-// the lane's row of a tensor.
-template <typename T, int D>
-__device__ __forceinline__ void store_row(const bl_heads &h, int64_t row, int64_t head, int half, uint32_t head_dim, const f32x16 (&acc)[D / 32],
+// Accumulators C[channel][the lane's row] of N blocks of 32 channels from
+// block `first` on, times `by`, to the lane's row of a tensor.
+template <typename T, int N>
+__device__ __forceinline__ void store_row(const bl_heads &h, int64_t row, int64_t head, int half, uint32_t head_dim, const f32x16 (&acc)[N], int first,
                                           float by) {
     typedef T T4 __attribute__((ext_vector_type(4)));
     T *at = (T *)h.data + row * (int64_t)h.row_stride + head * (int64_t)h.head_stride;
 #pragma unroll
-    for (int b = 0; b < D / 32; b++)
+    for (int b = 0; b < N; b++)
 #pragma unroll
         for (int r = 0; r < 16; r += 4) {
-            const uint32_t c = 32 * b + 2 * r + 4 * half;
+            const uint32_t c = 32 * (first + b) + 2 * r + 4 * half;
             T4 v;
 #pragma unroll
             for (int e = 0; e < 4; e++) v[e] = (T)(acc[b][r + e] * by);
             if (c < head_dim) *(T4 *)(at + c) = v;  // head_dim is a multiple of 8
         }
+}
+// The same to a row of a split's partial sums.
+template <int N>
+__device__ __forceinline__ void store_partial(float *at, int half, const f32x16 (&acc)[N], int first, float by) {
+#pragma unroll
+    for (int b = 0; b < N; b++)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4)
+            *(f32x4 *)(at + 32 * (first + b) + 2 * r + 4 * half) = f32x4{acc[b][r], acc[b][r + 1], acc[b][r + 2], acc[b][r + 3]} * by;
 }
 
 // ---- scores ----

@@ -12,23 +12,33 @@ uint64_t rounded(uint64_t bytes) { return (bytes + 255) / 256 * 256; }
 PackedPlan plan_packed(const bl_packed_attention_args &a, uint32_t compute_units) {
     PackedPlan plan{};
     plan.tile_dim = a.head_dim <= 64 ? 64 : 128;
-    const uint64_t group = a.q_heads / a.kv_heads;
-    // Workgroups of the forward without splits: 128 (row, head) places each.
-    const uint64_t whole = (a.q_rows * group / 128 + a.documents) * a.kv_heads;
+    const uint64_t group = a.q_heads / a.kv_heads, places = (uint64_t)a.q_rows * a.q_heads, key_places = (uint64_t)a.k_rows * a.kv_heads;
     const uint32_t keys = a.max_keys && a.max_keys < a.k_rows ? a.max_keys : a.k_rows;
-    // Few rows over many keys: the keys are split until the chip has four
-    // workgroups a compute unit, each with 256 keys or more.
-    const uint64_t wanted = whole ? 4ull * compute_units / whole : 1, most = (keys + 255) / 256;
-    plan.splits = (uint32_t)(wanted < most ? wanted : most);
-    if (plan.splits < 1) plan.splits = 1;
-    const uint64_t places = (uint64_t)a.q_rows * a.q_heads;
+    // Workgroups without splits: 128 (row, head) places or 128 keys each, and
+    // a last, partial one a document.
+    const uint64_t rows_whole = (a.q_rows * group / 128 + a.documents) * a.kv_heads;
+    const uint64_t keys_whole = ((uint64_t)a.k_rows / 128 + a.documents) * a.kv_heads;
+    // Few rows over much of the other side: that side is split until the chip
+    // has enough workgroups a compute unit, each with 256 streamed rows or more.
+    const auto splits = [&](uint64_t whole, uint32_t each, uint64_t streamed) {
+        const uint64_t wanted = whole ? (each * (uint64_t)compute_units + whole / 2) / whole : 1, most = (streamed + 255) / 256;
+        const uint64_t n = wanted < most ? wanted : most;
+        return (uint32_t)(n < 1 ? 1 : n > 1024 ? 1024 : n);
+    };
+    plan.splits = splits(rows_whole, 4, keys);
+    plan.splits_q = splits(rows_whole, 2, keys);
+    plan.splits_kv = splits(keys_whole, 2, (uint64_t)a.q_rows * group);
     if (plan.splits > 1) {
         plan.partial_bytes = rounded(plan.splits * places * plan.tile_dim * sizeof(float));
         plan.stats_bytes = rounded(plan.splits * places * 2 * sizeof(float));
     }
     plan.forward_bytes = plan.partial_bytes + plan.stats_bytes;
     plan.row_bytes = rounded(places * sizeof(float));
-    plan.backward_bytes = 3 * plan.row_bytes;
+    const uint64_t of_q = plan.splits_q > 1 ? plan.splits_q * 2 * places * plan.tile_dim * sizeof(float) : 0;
+    const uint64_t of_kv = plan.splits_kv > 1 ? plan.splits_kv * 2 * key_places * plan.tile_dim * sizeof(float) : 0;
+    plan.back_partial_bytes = rounded(of_q > of_kv ? of_q : of_kv);  // one after the other
+    plan.back_stats_bytes = plan.splits_q > 1 ? rounded(plan.splits_q * places * 4 * sizeof(float)) : 0;
+    plan.backward_bytes = 3 * plan.row_bytes + plan.back_partial_bytes + plan.back_stats_bytes;
     return plan;
 }
 
@@ -47,10 +57,13 @@ hipError_t launch_packed_forward(const PackedParams &q, const PackedPlan &plan, 
 hipError_t launch_packed_backward(const PackedParams &q, const PackedPlan &plan, hipStream_t s) {
     PackedParams p = q;
     char *at = (char *)p.a.workspace;
-    p.splits = 1;
+    p.splits_q = plan.splits_q;
+    p.splits_kv = plan.splits_kv;
     p.delta = (float *)at;
     p.largest = (float *)(at + plan.row_bytes);
-    p.d_slope = p.g.d_slopes ? (float *)(at + 2 * plan.row_bytes) : nullptr;
+    p.d_slope = (float *)(at + 2 * plan.row_bytes);
+    p.partial = (float *)(at + 3 * plan.row_bytes);
+    p.stats = (float *)(at + 3 * plan.row_bytes + plan.back_partial_bytes);
     switch (p.a.dtype) {
     case BL_F32: return packed_backward<float>(p, plan, s);
     case BL_F16: return packed_backward<_Float16>(p, plan, s);
