@@ -101,8 +101,11 @@ int check_attention(bl_ctx *ctx, const bl_packed_attention_args *a, const char *
     if (!std::isfinite(a->softcap) || a->softcap < 0.0f)
         return refuse(ctx, BL_ERR_INVALID_ARGUMENT, "%s: a softcap that is negative or not finite", what);
     // 32-bit places of the (row, head of a group) pairs, and of the tiles with one more per document.
+    // A grid has a workgroup for each 128 of them and each key head, and splits
+    // only where those are few.
     const uint64_t places = (uint64_t)a->q_rows * (a->q_heads / a->kv_heads);
-    if (places > 0x40000000ull || a->k_rows > 0x40000000u || a->documents > 0x01000000u || a->q_heads > 65535)
+    const uint64_t most = (places > a->k_rows ? places : a->k_rows) / 128 + a->documents;
+    if (places > 0x40000000ull || a->k_rows > 0x40000000u || a->documents > 0x01000000u || a->q_heads > 65535 || most * a->kv_heads > 0x40000000ull)
         return refuse(ctx, BL_ERR_TOO_LARGE, "%s: %u query rows of %u heads, %u key rows, %u documents", what, a->q_rows, a->q_heads,
                       a->k_rows, a->documents);
     return BL_OK;

@@ -17,6 +17,10 @@ constexpr float LN2 = 0.6931471805599453f;
 // branches want it there, and the compiler cannot always tell.
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
+__device__ __forceinline__ uint64_t uniform64(uint64_t v) {
+    return (uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32 | (uint32_t)uniform((int)v);
+}
+
 struct Document {
     int q0, n_q;     // first query row, query rows
     int k0, n_k;     // first key row, key rows
@@ -150,24 +154,23 @@ template <typename T, int D, int ROWS, int THREADS = 256> struct Tile {
 
     // Byte offsets of this thread's chunks from the tile's first row.
     uint32_t offset[LOADS];
-    uint32_t stride, end;  // bytes from a row to the next; of the last row
+    int stride, end;  // bytes from a row to the next; of the last row
 
     __device__ __forceinline__ Tile(uint64_t row_stride, uint32_t head_dim) {
-        stride = (uint32_t)row_stride * sizeof(T);
-        end = head_dim * sizeof(T);
+        stride = uniform((int)(row_stride * sizeof(T)));
+        end = uniform((int)(head_dim * sizeof(T)));
 #pragma unroll
         for (int n = 0; n < LOADS; n++) {
             const int i = n * THREADS + threadIdx.x;
             const int row = i / CHUNKS, chunk = (i % CHUNKS) ^ swizzle(row);
-            offset[n] = chunk * 16 < (int)end ? (uint32_t)row * stride + chunk * 16 : 0x7ffffff0u;
+            offset[n] = chunk * 16 < end ? (uint32_t)row * stride + chunk * 16 : 0x7ffffff0u;
         }
     }
-    // Starts the loads of up to `left` rows (at least one) from `base` into `lds`.
-    __device__ __forceinline__ void load(const char *base, int left, char *lds) const {
+    // Starts the loads of up to `left` rows (at least one) from `base` (a
+    // scalar address) into `lds`.
+    __device__ __forceinline__ void load(uint64_t base, int left, char *lds) const {
 #ifdef __HIP_DEVICE_COMPILE__  // the host pass knows no 16-byte loads to LDS
-        const uint32_t records = uniform((min(left, ROWS) - 1) * (int)stride + (int)end);
-        const uint64_t from = (uint64_t)(uint32_t)uniform((int)((uint64_t)base >> 32)) << 32 | (uint32_t)uniform((int)(uint64_t)base);
-        const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)from, 0, records, 0x00020000);
+        const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)uniform64(base), 0, uniform((min(left, ROWS) - 1) * stride + end), 0x00020000);
         const int wave = uniform(threadIdx.x / 64);
 #pragma unroll
         for (int n = 0; n < LOADS; n++)
@@ -230,6 +233,11 @@ template <typename T, int D, int ROWS, int BLOCKS = D / 32> struct Reader {
     }
 };
 
+// The address of a (row, head) of a tensor, scalar.
+template <typename T> __device__ __forceinline__ uint64_t address_of(const bl_heads &h, int64_t row, int64_t head) {
+    return uniform64((uint64_t)h.data + (uint64_t)(row * (int64_t)h.row_stride + head * (int64_t)h.head_stride) * sizeof(T));
+}
+
 // A lane's row of a tensor as operands along the channels, zeros beyond
 // head_dim and where the lane has none (`row` is then any row there is).
 template <typename T, int D>
@@ -278,38 +286,50 @@ __device__ __forceinline__ void store_partial(float *at, int half, const f32x16 
 // ---- scores ----
 //
 // In base two: x = log2(e) s, so probabilities are exp2(x - .). With a cap,
-// s = cap tanh(u), u = scale qk / cap.
+// s = cap tanh(u), u = scale qk / cap. `factor` is what x is of a product, or
+// of its tanh.
 
-struct ScoreConstants {
-    float scale2;    // log2(e) scale: x per qk, uncapped
-    float tanh2;     // 2 log2(e) scale / cap: the exponent of tanh's exponential per qk
-    float inner;     // scale / cap
-    float cap2;      // log2(e) cap
-    __device__ __forceinline__ explicit ScoreConstants(const bl_packed_attention_args &a) {
-        scale2 = a.scale * LOG2E;
-        inner = a.softcap > 0.0f ? a.scale / a.softcap : 0.0f;
-        tanh2 = 2.0f * LOG2E * inner;
-        cap2 = a.softcap * LOG2E;
+template <typename T, bool CAP> struct Scores {
+    float factor;  // log2(e) scale, or log2(e) cap
+    float inner;   // scale / cap
+    // `ordered`: for q whose sign the caller has changed where scale is
+    // negative, so that x grows with the product (and a scale of zero keeps a
+    // hidden -inf what it is).
+    __device__ __forceinline__ explicit Scores(const bl_packed_attention_args &a, bool ordered = false) {
+        const float scale = ordered ? fmaxf(fabsf(a.scale), 1e-37f) : a.scale;
+        factor = (CAP ? a.softcap : scale) * LOG2E;
+        inner = CAP ? scale / a.softcap : 0.0f;
+    }
+    // With a cap, products to their tanh u. f32 takes tanhf. For the 16-bit
+    // types a wave's tile of small u, the usual one (caps are wide), takes the
+    // odd series up to u^9, off by less than 2^-24 of tanh u for |u| < 0.3: 7
+    // operations, 28 cycles a wave; any other 1 - 2 / (e^2u + 1), off by a few
+    // steps of 1, with its two quarter-rate instructions 44.
+    __device__ __forceinline__ void caps(f32x16 &s) const {
+        if constexpr (!CAP) return;
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[r] = tanhf(s[r] * inner);
+        } else {
+            float top = 0.0f;
+#pragma unroll
+            for (int r = 0; r < 16; r += 2) top = fmaxf(fmaxf(fabsf(s[r]), fabsf(s[r + 1])), top);
+            if (__all(top * fabsf(inner) < 0.3f)) {  // a NaN is no maximum, and stays one in either form
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const float u = s[r] * inner, w = u * u;
+                    s[r] = u * (1.0f + w * (-1.0f / 3 + w * (2.0f / 15 + w * (-17.0f / 315 + w * (62.0f / 2835)))));
+                }
+            } else {
+                const float twice = 2.0f * LOG2E * inner;
+#pragma unroll
+                for (int r = 0; r < 16; r++) s[r] = 1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[r] * twice) + 1.0f);
+            }
+        }
     }
 };
 
-// x of one product, and with a cap its tanh. The 16-bit types take
-// tanh u = 1 - 2 / (e^2u + 1), good to a few steps of 1 (their own steps are
-// 2^13 and 2^16 times that); f32 takes tanhf, good to steps of the result.
-template <typename T, bool CAP>
-__device__ __forceinline__ float score(const ScoreConstants &k, float qk, float &th) {
-    if constexpr (!CAP) {
-        return qk * k.scale2;
-    } else if constexpr (sizeof(T) == 4) {
-        th = tanhf(qk * k.inner);
-        return th * k.cap2;
-    } else {
-        th = 1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(qk * k.tanh2) + 1.0f);
-        return th * k.cap2;
-    }
-}
-
-// Sum over axes of |a - b|, axes beyond `axes` left out.
-__device__ __forceinline__ uint32_t apart(int a, int b) { return a > b ? (uint32_t)a - (uint32_t)b : (uint32_t)b - (uint32_t)a; }
+// |a - b| + c of values whose order is that of unsigned numbers: one v_sad_u32.
+__device__ __forceinline__ uint32_t apart(uint32_t a, uint32_t b, uint32_t c) { return (max(a, b) - min(a, b)) + c; }
 
 }  // namespace bl
