@@ -57,7 +57,7 @@ int check_vector(bl_ctx *ctx, const void *p, uint64_t size, const char *what, co
 }
 
 uint64_t norm_workspace(bl_ctx *ctx, const bl_layer_norm_args *a) {
-    return (uint64_t)bl::norm_groups(a->rows, a->cols, bl_compute_units_of(ctx)) * 2 * a->cols * sizeof(float);
+    return (uint64_t)bl::norm_groups(a->rows, a->cols, bl_compute_units_of(ctx), bl::NORM_BACKWARD_GROUPS) * 2 * a->cols * sizeof(float);
 }
 
 // ---- views [rows][heads][head_dim] ----
@@ -169,8 +169,7 @@ extern "C" int bl_layer_norm(bl_ctx *ctx, const bl_layer_norm_args *a) {
     p.rows = a->rows;
     p.cols = a->cols;
     p.epsilon = a->epsilon;
-    p.vector = a->cols * size % 16 == 0 && a->x_stride * size % 16 == 0 && a->y_stride * size % 16 == 0 && aligned(a->x, 16) &&
-               aligned(a->y, 16) && aligned(a->gamma, 16) && aligned(a->beta, 16);
+    p.groups = bl::norm_groups(a->rows, a->cols, bl_compute_units_of(ctx), bl::NORM_FORWARD_GROUPS);
     const DeviceScope scope(bl_device_of(ctx));
     if (scope.status != hipSuccess) return launched(ctx, scope.status, what);
     return launched(ctx, bl::launch_norm_forward(p, a->dtype, bl_stream_of(ctx)), what);
@@ -223,9 +222,7 @@ extern "C" int bl_layer_norm_backward(bl_ctx *ctx, const bl_layer_norm_args *a, 
     p.dx_stride = g->dx_stride;
     p.rows = a->rows;
     p.cols = a->cols;
-    p.groups = bl::norm_groups(a->rows, a->cols, bl_compute_units_of(ctx));
-    p.vector = a->cols * size % 16 == 0 && a->x_stride * size % 16 == 0 && g->dy_stride * size % 16 == 0 && g->dx_stride * size % 16 == 0 &&
-               aligned(a->x, 16) && aligned(g->dy, 16) && aligned(g->dx, 16) && aligned(a->gamma, 16);
+    p.groups = bl::norm_groups(a->rows, a->cols, bl_compute_units_of(ctx), bl::NORM_BACKWARD_GROUPS);
     const DeviceScope scope(bl_device_of(ctx));
     if (scope.status != hipSuccess) return launched(ctx, scope.status, what);
     return launched(ctx, bl::launch_norm_backward(p, a->dtype, bl_stream_of(ctx)), what);

@@ -19,10 +19,11 @@ struct NormParams {
     uint64_t x_stride, y_stride, dy_stride, dx_stride;
     uint32_t rows, cols, groups;
     float epsilon;
-    bool vector;  // every row of every tensor starts at 16 bytes and holds whole 16-byte chunks
 };
-// Workgroups of the backward: what its workspace holds a partial sum of each for.
-uint32_t norm_groups(uint32_t rows, uint32_t cols, uint32_t compute_units);
+// Workgroups that walk the rows, up to `each` of 256 threads a compute unit.
+// The backward's workspace holds a partial sum of each.
+uint32_t norm_groups(uint32_t rows, uint32_t cols, uint32_t compute_units, uint32_t each);
+constexpr uint32_t NORM_FORWARD_GROUPS = 8, NORM_BACKWARD_GROUPS = 3;
 hipError_t launch_norm_forward(const NormParams &p, uint32_t dtype, hipStream_t s);
 hipError_t launch_norm_backward(const NormParams &p, uint32_t dtype, hipStream_t s);
 

@@ -98,7 +98,7 @@ extern "C" hipError_t hipSetDevice(int) { return hipSuccess; }
 extern "C" const char *hipGetErrorString(hipError_t) { return ""; }
 namespace bl {
 static hipError_t launch() { the_ctx.launches++; return hipSuccess; }
-uint32_t norm_groups(uint32_t rows, uint32_t, uint32_t) { return rows ? 1 : 0; }
+uint32_t norm_groups(uint32_t rows, uint32_t, uint32_t, uint32_t) { return rows ? 1 : 0; }
 hipError_t launch_norm_forward(const NormParams &, uint32_t, hipStream_t) { return launch(); }
 hipError_t launch_norm_backward(const NormParams &, uint32_t, hipStream_t) { return launch(); }
 hipError_t launch_rotary(const RotaryParams &, uint32_t, uint32_t, hipStream_t) { return launch(); }
