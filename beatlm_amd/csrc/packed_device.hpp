@@ -300,31 +300,43 @@ template <typename T, bool CAP> struct Scores {
         factor = (CAP ? a.softcap : scale) * LOG2E;
         inner = CAP ? scale / a.softcap : 0.0f;
     }
-    // With a cap, products to their tanh u. f32 takes tanhf. For the 16-bit
-    // types a wave's tile of small u, the usual one (caps are wide), takes the
-    // odd series up to u^9, off by less than 2^-24 of tanh u for |u| < 0.3: 7
-    // operations, 28 cycles a wave; any other 1 - 2 / (e^2u + 1), off by a few
-    // steps of 1, with its two quarter-rate instructions 44.
+    // With a cap, products to their tanh u. Where a wave's tile has no |u| of
+    // LIMIT or more, the usual case as caps are wide, a polynomial in u^2
+    // (fitted to tanh(u) / u at Chebyshev points) that is off by less than a
+    // step of f32: 4 or 7 multiplications more than the product itself, 28
+    // cycles a wave for the 16-bit types. Any other tile: 1 - 2 / (e^2u + 1),
+    // off by a few steps of 1, 44 cycles with its two quarter-rate
+    // instructions; f32 takes tanhf, some ten times that.
     __device__ __forceinline__ void caps(f32x16 &s) const {
         if constexpr (!CAP) return;
-        if constexpr (sizeof(T) == 4) {
+        constexpr bool F32 = sizeof(T) == 4;
+        constexpr float LIMIT = F32 ? 1.0f : 0.5f;
+        float top = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) top = fmaxf(fmaxf(fabsf(s[r]), fabsf(s[r + 1])), top);
+        if (__all(top * fabsf(inner) < LIMIT)) {  // a NaN is no maximum, and stays one in either form
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const float u = s[r] * inner, w = u * u;
+                float v;
+                if constexpr (F32) {
+                    v = 0.00228764559f + w * -0.000354883407f;
+                    v = 0.0214699805f + w * (-0.00792494603f + w * v);
+                    v = 0.133321911f + w * (-0.053872738f + w * v);
+                    v = 1.0f + w * (-0.333332807f + w * v);
+                } else {
+                    v = 0.133248284f + w * (-0.0529892407f + w * 0.0171413198f);
+                    v = 1.0f + w * (-0.333330721f + w * v);
+                }
+                s[r] = u * v;
+            }
+        } else if constexpr (F32) {
 #pragma unroll
             for (int r = 0; r < 16; r++) s[r] = tanhf(s[r] * inner);
         } else {
-            float top = 0.0f;
+            const float twice = 2.0f * LOG2E * inner;
 #pragma unroll
-            for (int r = 0; r < 16; r += 2) top = fmaxf(fmaxf(fabsf(s[r]), fabsf(s[r + 1])), top);
-            if (__all(top * fabsf(inner) < 0.3f)) {  // a NaN is no maximum, and stays one in either form
-#pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    const float u = s[r] * inner, w = u * u;
-                    s[r] = u * (1.0f + w * (-1.0f / 3 + w * (2.0f / 15 + w * (-17.0f / 315 + w * (62.0f / 2835)))));
-                }
-            } else {
-                const float twice = 2.0f * LOG2E * inner;
-#pragma unroll
-                for (int r = 0; r < 16; r++) s[r] = 1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[r] * twice) + 1.0f);
-            }
+            for (int r = 0; r < 16; r++) s[r] = 1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[r] * twice) + 1.0f);
         }
     }
 };
