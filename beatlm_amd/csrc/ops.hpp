@@ -42,12 +42,16 @@ hipError_t launch_rotary(const RotaryParams &p, uint32_t dtype, uint32_t compute
 
 // ---- attention over packed documents ----
 
+// (row, head of a group) places, or keys, of a workgroup.
+constexpr int ROWS = 128, FEW_ROWS = 32;
+
 struct PackedParams {
     bl_packed_attention_args a;
     bl_packed_attention_grads g;
     // Where the streamed side is split over workgroups, each split's sums,
     // joined by a launch of its own.
     uint32_t splits, splits_q, splits_kv;
+    bool few;        // the forward's workgroups have FEW_ROWS places, not ROWS
     float *partial;  // forward [splits][places][tile_dim]; d_q [splits][2][places][tile_dim]; d_k, d_v [splits][2][k_rows * kv_heads][tile_dim]
     float *stats;    // forward [splits][places][2], d_q [splits][places][4]; places = q_rows * q_heads
     // backward, [q_heads][q_rows] each
@@ -57,6 +61,7 @@ struct PackedParams {
 };
 struct PackedPlan {
     uint32_t splits, splits_q, splits_kv;
+    bool few;
     uint32_t tile_dim;  // channels of the kernels' tiles: 64 or 128
     uint64_t partial_bytes, stats_bytes;                     // forward
     uint64_t row_bytes, back_partial_bytes, back_stats_bytes; // backward

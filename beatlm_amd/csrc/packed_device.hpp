@@ -161,20 +161,21 @@ template <typename T, int D, int ROWS, int THREADS = 256> struct Tile {
         end = uniform((int)(head_dim * sizeof(T)));
 #pragma unroll
         for (int n = 0; n < LOADS; n++) {
-            const int i = n * THREADS + threadIdx.x;
+            const int i = n * THREADS + threadIdx.x % THREADS;
             const int row = i / CHUNKS, chunk = (i % CHUNKS) ^ swizzle(row);
             offset[n] = chunk * 16 < end ? (uint32_t)row * stride + chunk * 16 : 0x7ffffff0u;
         }
     }
-    // Starts the loads of up to `left` rows (at least one) from `base` (a
-    // scalar address) into `lds`.
-    __device__ __forceinline__ void load(uint64_t base, int left, char *lds) const {
+    // Starts the loads of up to `left` rows from `base` (a scalar address)
+    // into `lds`, zeros where there are none; `own`: bytes on, where the loading threads
+    // are one wave of several with a tile each.
+    __device__ __forceinline__ void load(uint64_t base, int left, char *lds, int own = 0) const {
 #ifdef __HIP_DEVICE_COMPILE__  // the host pass knows no 16-byte loads to LDS
-        const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)uniform64(base), 0, uniform((min(left, ROWS) - 1) * stride + end), 0x00020000);
-        const int wave = uniform(threadIdx.x / 64);
+        const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)uniform64(base), 0, uniform(left > 0 ? (min(left, ROWS) - 1) * stride + end : 0), 0x00020000);
+        const int wave = uniform(threadIdx.x % THREADS / 64);
 #pragma unroll
         for (int n = 0; n < LOADS; n++)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void *)(lds + (n * THREADS + wave * 64) * 16), 16,
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void *)(lds + own + (n * THREADS + wave * 64) * 16), 16,
                                                      offset[n], 0, 0, 0);
 #endif
     }

@@ -16,8 +16,8 @@ PackedPlan plan_packed(const bl_packed_attention_args &a, uint32_t compute_units
     const uint32_t keys = a.max_keys && a.max_keys < a.k_rows ? a.max_keys : a.k_rows;
     // Workgroups without splits: 128 (row, head) places or 128 keys each, and
     // a last, partial one a document.
-    const uint64_t rows_whole = (a.q_rows * group / 128 + a.documents) * a.kv_heads;
-    const uint64_t keys_whole = ((uint64_t)a.k_rows / 128 + a.documents) * a.kv_heads;
+    const uint64_t rows_whole = (a.q_rows * group / ROWS + a.documents) * a.kv_heads;
+    const uint64_t keys_whole = ((uint64_t)a.k_rows / ROWS + a.documents) * a.kv_heads;
     // The streamed side is split where there are few workgroups, each split
     // keeping 64 streamed rows or more. The forward splits where the chip is
     // not covered once, then to four workgroups a compute unit (16 tokens over
@@ -31,7 +31,11 @@ PackedPlan plan_packed(const bl_packed_attention_args &a, uint32_t compute_units
         return (uint32_t)(n < 1 ? 1 : n > 1024 ? 1024 : n);
     };
     const auto twice = [&](uint64_t whole) { return whole ? (2 * units + whole / 2) / whole : 1; };
-    plan.splits = splits(rows_whole && rows_whole < units ? 4 * units / rows_whole : 1, keys);
+    // Documents of few places, 32 on average at most: workgroups of 32, where
+    // there is a kernel for them (heads of up to 64 in f32).
+    plan.few = a.dtype == BL_F32 && plan.tile_dim == 64 && (uint64_t)a.q_rows * group <= (uint64_t)FEW_ROWS * a.documents;
+    const uint64_t forward_whole = plan.few ? ((uint64_t)a.q_rows * group / FEW_ROWS + a.documents) * a.kv_heads : rows_whole;
+    plan.splits = splits(forward_whole && forward_whole < units ? (plan.few ? 2 : 4) * units / forward_whole : 1, keys);
     plan.splits_q = splits(twice(rows_whole), keys);
     plan.splits_kv = splits(twice(keys_whole), (uint64_t)a.q_rows * group);
     if (plan.splits > 1) {
@@ -51,6 +55,7 @@ PackedPlan plan_packed(const bl_packed_attention_args &a, uint32_t compute_units
 hipError_t launch_packed_forward(const PackedParams &q, const PackedPlan &plan, hipStream_t s) {
     PackedParams p = q;
     p.splits = plan.splits;
+    p.few = plan.few;
     p.partial = (float *)p.a.workspace;
     p.stats = (float *)((char *)p.a.workspace + plan.partial_bytes);
     switch (p.a.dtype) {
