@@ -1,7 +1,7 @@
 // LayerNorm over strided rows and its gradients (include/beatlm_ops.h).
 //
-// Both directions read each row once: TPR threads (one wave, four or sixteen)
-// keep it in registers, 16 values each, so the variance is the mean of squares
+// Both directions read each row once: TPR threads (a quarter of a wave to
+// sixteen waves) keep it in registers, 16 values each, so the variance is the mean of squares
 // about the mean (two passes over registers, no cancellation) and nothing is
 // read twice. The bound is HBM: forward x in, y out; backward x and dy in, dx
 // out. Rows come and go in 16-byte pieces wherever they start (the memory
@@ -20,7 +20,7 @@ namespace bl {
 namespace {
 
 constexpr int EPT = 16;  // values of a row a thread holds
-template <int TPR> constexpr int norm_threads = TPR == 64 ? 256 : TPR;  // of a workgroup
+template <int TPR> constexpr int norm_threads = TPR <= 64 ? 256 : TPR;  // of a workgroup
 
 // Sum over the wave, in every lane, without LDS: 16 lanes by DPP, then the
 // two exchanges of rows of 16 and of 32.
@@ -34,7 +34,7 @@ __device__ __forceinline__ float wave_sum_dpp(float v) {
 template <int TPR, int K>
 __device__ __forceinline__ void row_sums(float (&v)[K], float *lds) {
 #pragma unroll
-    for (int k = 0; k < K; k++) v[k] = wave_sum_dpp(v[k]);
+    for (int k = 0; k < K; k++) v[k] = TPR == 16 ? row16_sum(v[k]) : wave_sum_dpp(v[k]);
     if constexpr (TPR > 64) {
         constexpr int WAVES = TPR / 64;
         const int wave = threadIdx.x / 64;
@@ -90,10 +90,10 @@ template <typename T, int TPR>
 __global__ __launch_bounds__(norm_threads<TPR>) void norm_forward_kernel(NormParams p) {
     typedef Pieces<T, TPR> P;
     constexpr int VEC = P::VEC, N = P::N, ROWS = norm_threads<TPR> / TPR;
-    __shared__ float lds[TPR / 64];
+    __shared__ float lds[TPR / 64 + 1];
     const int lane = threadIdx.x % TPR;
     uint32_t row = blockIdx.x * ROWS + threadIdx.x / TPR;
-    if (row >= p.rows) return;  // whole waves of a one-wave row; no barrier follows for those
+    if (row >= p.rows) return;  // all threads of a row; with rows of a wave or less no barrier follows
     P x, gamma, beta;
     x.load((const T *)p.x + (uint64_t)row * p.x_stride, p.cols, lane, (T)0.0f);
     gamma.load((const T *)p.gamma, p.cols, lane, (T)0.0f);
@@ -139,7 +139,7 @@ template <typename T, int TPR>
 __global__ __launch_bounds__(norm_threads<TPR>) void norm_backward_kernel(NormParams p) {
     typedef Pieces<T, TPR> P;
     constexpr int VEC = P::VEC, N = P::N, ROWS = norm_threads<TPR> / TPR, WIDTH = TPR * EPT;
-    __shared__ float lds[TPR == 64 ? 2 * ROWS * WIDTH : 2 * (TPR / 64)];
+    __shared__ float lds[TPR <= 64 ? 2 * ROWS * WIDTH : 2 * (TPR / 64)];
     const int lane = threadIdx.x % TPR;
     P gamma, x, dy;
     gamma.load((const T *)p.gamma, p.cols, lane, (T)0.0f);
@@ -190,16 +190,16 @@ __global__ __launch_bounds__(norm_threads<TPR>) void norm_backward_kernel(NormPa
             P::store(dx, p.cols, lane, n, out);
         }
     }
-    // The workgroup's partial sums; of one-wave rows, the waves' added first.
+    // The workgroup's partial sums; where it has several rows at once, theirs added first.
     float *out = p.partial + (uint64_t)blockIdx.x * 2 * p.cols;
-    if constexpr (TPR == 64) {
-        const int wave = threadIdx.x / 64;
+    if constexpr (TPR <= 64) {
+        const int which_row = threadIdx.x / TPR;
 #pragma unroll
         for (int n = 0; n < N; n++)
 #pragma unroll
             for (int e = 0; e < VEC; e++) {
-                lds[(wave * 2 + 0) * WIDTH + P::col(lane, n) + e] = dg[n][e];
-                lds[(wave * 2 + 1) * WIDTH + P::col(lane, n) + e] = db[n][e];
+                lds[(which_row * 2 + 0) * WIDTH + P::col(lane, n) + e] = dg[n][e];
+                lds[(which_row * 2 + 1) * WIDTH + P::col(lane, n) + e] = db[n][e];
             }
         __syncthreads();
         for (uint32_t i = threadIdx.x; i < 2 * p.cols; i += 256) {
@@ -254,13 +254,15 @@ __global__ __launch_bounds__(1024) void norm_reduce_kernel(NormParams p) {
     else p.d_beta[i - p.cols] = s;
 }
 
-// The threads a row of `cols` gets: a wave for up to 1024 columns, four for up
-// to 4096, sixteen for the rest.
-uint32_t threads_per_row(uint32_t cols) { return cols <= 64 * EPT ? 64 : cols <= 256 * EPT ? 256 : 1024; }
+// The threads a row of `cols` gets: a quarter of a wave for up to 256 columns
+// (forward and backward of 8353 x 128 bf16 12.5 us, with a wave 20.8), a wave
+// for up to 1024, four for up to 4096, sixteen for the rest.
+uint32_t threads_per_row(uint32_t cols) { return cols <= 16 * EPT ? 16 : cols <= 64 * EPT ? 64 : cols <= 256 * EPT ? 256 : 1024; }
 
 template <typename T>
 hipError_t forward(const NormParams &p, hipStream_t s) {
     switch (threads_per_row(p.cols)) {
+    case 16: norm_forward_kernel<T, 16><<<p.groups, 256, 0, s>>>(p); break;
     case 64: norm_forward_kernel<T, 64><<<p.groups, 256, 0, s>>>(p); break;
     case 256: norm_forward_kernel<T, 256><<<p.groups, 256, 0, s>>>(p); break;
     default: norm_forward_kernel<T, 1024><<<p.groups, 1024, 0, s>>>(p); break;
@@ -272,6 +274,7 @@ template <typename T>
 hipError_t backward(const NormParams &p, hipStream_t s) {
     if (p.groups) {
         switch (threads_per_row(p.cols)) {
+        case 16: norm_backward_kernel<T, 16><<<p.groups, 256, 0, s>>>(p); break;
         case 64: norm_backward_kernel<T, 64><<<p.groups, 256, 0, s>>>(p); break;
         case 256: norm_backward_kernel<T, 256><<<p.groups, 256, 0, s>>>(p); break;
         default: norm_backward_kernel<T, 1024><<<p.groups, 1024, 0, s>>>(p); break;
@@ -286,7 +289,7 @@ hipError_t backward(const NormParams &p, hipStream_t s) {
 }  // namespace
 
 uint32_t norm_groups(uint32_t rows, uint32_t cols, uint32_t compute_units, uint32_t each) {
-    const uint32_t threads = threads_per_row(cols), at_once = threads == 64 ? 4 : 1;
+    const uint32_t threads = threads_per_row(cols), at_once = threads <= 64 ? 256 / threads : 1;
     const uint64_t most = (uint64_t)compute_units * (threads == 1024 ? (each + 3) / 4 : each), need = ((uint64_t)rows + at_once - 1) / at_once;
     return (uint32_t)(need < most ? need : most);
 }
