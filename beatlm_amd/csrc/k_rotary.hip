@@ -17,6 +17,7 @@ struct RotaryGeometry {
     uint32_t pair_units;
     uint32_t head_groups;  // threads that share a row's heads
     uint32_t rows;         // rows a workgroup holds at once
+    uint32_t first;        // the launch's first row
 };
 
 template <typename T, int VEC>
@@ -72,7 +73,7 @@ template <typename T, int VEC>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p, RotaryGeometry geo) {
     const uint32_t unit = threadIdx.x % geo.units, rest = threadIdx.x / geo.units;
     const uint32_t group = rest % geo.head_groups, slot = rest / geo.head_groups;
-    const uint64_t at = (uint64_t)blockIdx.x * geo.rows + slot;
+    const uint64_t at = geo.first + (uint64_t)blockIdx.x * geo.rows + slot;
     if (slot >= geo.rows || at >= p.rows) return;
     const uint32_t row = (uint32_t)at;
     float co[VEC], si[VEC];
@@ -103,8 +104,14 @@ hipError_t launch(const RotaryParams &p, uint32_t compute_units, hipStream_t s) 
            p.rows < 2ull * compute_units * (256 / (g.units * g.head_groups)))
         g.head_groups *= 2;
     g.rows = 256 / (g.units * g.head_groups);
-    rotary_kernel<T, VEC><<<(p.rows + g.rows - 1) / g.rows, 256, 0, s>>>(p, g);
-    return hipGetLastError();
+    // A grid has fewer than 2^32 threads: more rows than that take more launches.
+    const uint64_t most = 1u << 23, groups = ((uint64_t)p.rows + g.rows - 1) / g.rows;
+    for (uint64_t done = 0; done < groups; done += most) {
+        g.first = (uint32_t)(done * g.rows);
+        rotary_kernel<T, VEC><<<(uint32_t)(groups - done < most ? groups - done : most), 256, 0, s>>>(p, g);
+        if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace

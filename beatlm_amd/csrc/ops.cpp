@@ -75,7 +75,11 @@ struct HeadsCheck {
         if (!aligned(h.data, align) || (rows > 1 && h.row_stride * size % align) || (heads > 1 && h.head_stride * size % align))
             return refuse(ctx, BL_ERR_MISALIGNED_PLACEMENT, "%s: %s's address or strides are not multiples of %llu bytes", what, name,
                           (unsigned long long)align);
-        if (written && ((rows > 1 && h.row_stride < head_dim) || (heads > 1 && h.head_stride < head_dim)))
+        // Rows of all heads, or heads of all rows: either lies in one step of the other.
+        const auto apart = [&](uint64_t step, uint64_t n, uint64_t inner, uint64_t m) {
+            return n <= 1 || (step >= head_dim && (m <= 1 || inner > step || step >= (m - 1) * inner + head_dim));
+        };
+        if (written && (!apart(h.row_stride, rows, h.head_stride, heads) || !apart(h.head_stride, heads, h.row_stride, rows)))
             return refuse(ctx, BL_ERR_INVALID_ARGUMENT, "%s: %s's heads of %u overlap", what, name, head_dim);
         // Within a tile of 128 rows, bytes are addressed by 32-bit offsets.
         if ((rows > 1 && h.row_stride > (1u << 24) / size) || (heads > 1 && h.head_stride > (1ull << 40)))
@@ -100,14 +104,37 @@ int check_attention(bl_ctx *ctx, const bl_packed_attention_args *a, const char *
     if (!std::isfinite(a->scale)) return refuse(ctx, BL_ERR_INVALID_ARGUMENT, "%s: non-finite scale", what);
     if (!std::isfinite(a->softcap) || a->softcap < 0.0f)
         return refuse(ctx, BL_ERR_INVALID_ARGUMENT, "%s: a softcap that is negative or not finite", what);
+    // What the scores are multiplied by, in base two and under the cap.
+    const float log2e = 1.4426950408889634f;
+    if (!std::isfinite(a->scale * log2e) || !std::isfinite(a->softcap * log2e) || (a->softcap > 0.0f && !std::isfinite(2.0f * log2e * a->scale / a->softcap)))
+        return refuse(ctx, BL_ERR_INVALID_ARGUMENT, "%s: a scale of %g under a softcap of %g is beyond f32", what, a->scale, a->softcap);
     // 32-bit places of the (row, head of a group) pairs, and of the tiles with one more per document.
-    // A grid has a workgroup for each 128 of them and each key head, and splits
-    // only where those are few.
+    // A grid has a workgroup of up to 512 threads for each 128 of them and each
+    // key head (splits only where those are few), and fewer than 2^32 threads.
     const uint64_t places = (uint64_t)a->q_rows * (a->q_heads / a->kv_heads);
     const uint64_t most = (places > a->k_rows ? places : a->k_rows) / 128 + a->documents;
-    if (places > 0x40000000ull || a->k_rows > 0x40000000u || a->documents > 0x01000000u || a->q_heads > 65535 || most * a->kv_heads > 0x40000000ull)
+    if (places > 0x40000000ull || a->k_rows > 0x40000000u || a->documents > 0x01000000u || a->q_heads > 65535 || most * a->kv_heads > 0x7fffffull)
         return refuse(ctx, BL_ERR_TOO_LARGE, "%s: %u query rows of %u heads, %u key rows, %u documents", what, a->q_rows, a->q_heads,
                       a->k_rows, a->documents);
+    return BL_OK;
+}
+
+// A tensor that a call writes starts where none of the others does.
+struct Named {
+    const bl_heads &h;
+    uint32_t rows;
+    const char *name;
+};
+template <size_t N, size_t M>
+int check_separate(bl_ctx *ctx, const char *what, const Named (&written)[N], const Named (&read)[M]) {
+    for (size_t i = 0; i < N; i++) {
+        const Named &w = written[i];
+        for (size_t j = 0; j < i + M; j++) {
+            const Named &r = j < i ? written[j] : read[j - i];
+            if (w.rows && r.rows && w.h.data == r.h.data)
+                return refuse(ctx, BL_ERR_INVALID_ARGUMENT, "%s: %s is %s", what, w.name, r.name);
+        }
+    }
     return BL_OK;
 }
 
@@ -269,17 +296,17 @@ extern "C" int bl_rotary(bl_ctx *ctx, const bl_rotary_table *t, const bl_rotary_
     if (a->rows && (!a->positions || !aligned(a->positions, 4)))
         return refuse(ctx, BL_ERR_INVALID_ARGUMENT, "%s: positions are null or misaligned", what);
     const uint64_t size = element_size(a->dtype);
+    const auto same = [&](const bl_heads &x, const bl_heads &y) {
+        return x.data == y.data && x.row_stride == y.row_stride && x.head_stride == y.head_stride;
+    };
+    if ((a->q_heads && a->q_in.data && a->q_in.data == a->q_out.data && !same(a->q_in, a->q_out)) ||
+        (a->k_heads && a->k_in.data && a->k_in.data == a->k_out.data && !same(a->k_in, a->k_out)))
+        return refuse(ctx, BL_ERR_INVALID_ARGUMENT, "%s: an output is its input with other strides", what);
     const HeadsCheck heads{ctx, what, a->dtype, a->head_dim, size};
     if (int rc = heads(a->q_in, a->rows, a->q_heads, false, "q_in")) return rc;
     if (int rc = heads(a->q_out, a->rows, a->q_heads, true, "q_out")) return rc;
     if (int rc = heads(a->k_in, a->rows, a->k_heads, false, "k_in")) return rc;
     if (int rc = heads(a->k_out, a->rows, a->k_heads, true, "k_out")) return rc;
-    const auto same = [&](const bl_heads &x, const bl_heads &y) {
-        return x.data == y.data && x.row_stride == y.row_stride && x.head_stride == y.head_stride;
-    };
-    if ((a->q_heads && a->q_in.data == a->q_out.data && !same(a->q_in, a->q_out)) ||
-        (a->k_heads && a->k_in.data == a->k_out.data && !same(a->k_in, a->k_out)))
-        return refuse(ctx, BL_ERR_INVALID_ARGUMENT, "%s: an output is its input with other strides", what);
     if (a->rows == 0) return BL_OK;
     bl::RotaryParams p{};
     p.table = *t;
@@ -322,6 +349,8 @@ extern "C" int bl_packed_attention(bl_ctx *ctx, const bl_packed_attention_args *
     if (!ctx) return BL_ERR_INVALID_ARGUMENT;
     if (int rc = check_attention(ctx, a, what)) return rc;
     if (int rc = check_attention_arrays(ctx, a, what)) return rc;
+    const Named out[] = {{a->out, a->q_rows, "out"}}, in[] = {{a->q, a->q_rows, "q"}, {a->k, a->k_rows, "k"}, {a->v, a->k_rows, "v"}};
+    if (int rc = check_separate(ctx, what, out, in)) return rc;
     const bl::PackedPlan plan = bl::plan_packed(*a, bl_compute_units_of(ctx));
     if (int rc = check_workspace(ctx, a, plan.forward_bytes, what)) return rc;
     if (a->q_rows == 0) return BL_OK;
@@ -348,6 +377,9 @@ extern "C" int bl_packed_attention_backward(bl_ctx *ctx, const bl_packed_attenti
     if (int rc = heads(g->d_q, a->q_rows, a->q_heads, true, "d_q")) return rc;
     if (int rc = heads(g->d_k, a->k_rows, a->kv_heads, true, "d_k")) return rc;
     if (int rc = heads(g->d_v, a->k_rows, a->kv_heads, true, "d_v")) return rc;
+    const Named grads[] = {{g->d_q, a->q_rows, "d_q"}, {g->d_k, a->k_rows, "d_k"}, {g->d_v, a->k_rows, "d_v"}};
+    const Named in[] = {{a->q, a->q_rows, "q"}, {a->k, a->k_rows, "k"}, {a->v, a->k_rows, "v"}, {a->out, a->q_rows, "out"}, {g->d_out, a->q_rows, "d_out"}};
+    if (int rc = check_separate(ctx, what, grads, in)) return rc;
     const bl::PackedPlan plan = bl::plan_packed(*a, bl_compute_units_of(ctx));
     if (int rc = check_workspace(ctx, a, plan.backward_bytes, what)) return rc;
     bl::PackedParams p{};

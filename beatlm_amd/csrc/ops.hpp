@@ -1,6 +1,6 @@
 // The packed attention sublayer's operators (include/beatlm_ops.h): what the
-// host side (ops.cpp) hands to the kernels (k_norm.hip, k_rotary.hip,
-// k_packed.hip). Every launch function checks nothing: ops.cpp has.
+// host side (ops.cpp, packed_plan.cpp) hands to the kernels (k_norm.hip,
+// k_rotary.hip, k_packed.inc). The launch functions check nothing: ops.cpp has.
 #pragma once
 
 #include <hip/hip_runtime.h>

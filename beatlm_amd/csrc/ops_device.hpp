@@ -8,10 +8,6 @@
 
 namespace bl {
 
-template <typename T> struct Chunk { static constexpr int N = 16 / sizeof(T); };
-
-template <typename T> __device__ __forceinline__ float as_f32(T v) { return (float)v; }
-
 // VEC elements at p (16-byte aligned when VEC > 1) as f32.
 template <typename T, int VEC>
 __device__ __forceinline__ void load_vec(const T *p, float (&v)[VEC]) {

@@ -169,8 +169,9 @@ int bl_rotary(bl_ctx *ctx, const bl_rotary_table *table, const bl_rotary_args *a
  * no document are not touched, neither in out and lse nor in the gradients;
  * memory outside the documents is never read, so it may hold anything. Hidden
  * scores count as exactly -inf whatever q and k hold there; a hidden key's v
- * may be anything too. Sums, statistics and scores are f32; the probabilities
- * are rounded to the tensors' type for the product with v (f32 stays f32).
+ * may be anything too. Sums, statistics and scores are f32; for the matrix
+ * cores the probabilities, and the scores' gradients, are rounded to the
+ * tensors' type (f32 stays f32). What a call writes overlaps nothing else.
  *
  * The offsets are device arrays, read when the kernels run (a captured graph
  * may be replayed with others); they are clamped to the tensors' rows, so
@@ -181,7 +182,9 @@ int bl_rotary(bl_ctx *ctx, const bl_rotary_table *table, const bl_rotary_args *a
  * into their shared key head, and d_slopes summed over rows; fixed order of
  * sums, so equal calls give equal bits. It takes the keys packed by one array
  * of offsets (k_end = k_begin + 1), as documents that shared keys would have
- * to add to each other's gradients.
+ * to add to each other's gradients. A document whose q, k, v or d_out holds a
+ * NaN or an infinity, hidden or not, has gradients that mean nothing, and so
+ * do d_slopes of its heads; the other documents' are their own.
  * ------------------------------------------------------------------------ */
 #define BL_ATTENTION_MAX_HEAD_DIM 128u
 enum { BL_MASK_NONE = 0, BL_MASK_CAUSAL = 1, BL_MASK_PREFIX = 2 };

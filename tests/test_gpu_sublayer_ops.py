@@ -586,3 +586,170 @@ def test_a_sublayer_s_training_step(gpu, dtype):
     for name, got, w in (("out", out, o.detach()), ("dx", dx, want[0]), ("d_gamma", d_gamma, want[1]), ("d_beta", d_beta, want[2]), ("d_slopes", d_slopes, want[3])):
         off = float((got.double().cpu() - w).norm() / w.norm())
         assert off <= most, (name, off, most)
+
+
+# ---------------------------------------------------------------------------
+# where it can go wrong
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("mask", ["none", "causal"])
+def test_a_single_key_takes_all_the_weight(gpu, dtype, d, mask):
+    """One visible key: its value comes out as it is, and no gradient reaches
+    the scores, exactly."""
+    t = Packed([(1, 1)] * 70 + [(7, 1) if mask == "none" else (1, 1)], dtype, 4, 2, d, mask=mask, cap=9.0, bias=0.2)
+    a = t.args(gpu, True)
+    ops.attention(gpu, a)
+    ops.attention_backward(gpu, a, t.grads())
+    t.check(["out", "lse", "d_v"], True)
+    assert torch.equal(t.out[:70], t.v[:70].repeat_interleave(2, 1))
+    for grad in (t.d_q, t.d_k, t.d_slopes):
+        assert torch.all(grad == 0.0)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("mask,prefix", [("causal", None), ("prefix", [1, 0])])
+def test_rows_of_one_key_or_none_among_others(gpu, dtype, mask, prefix):
+    """More queries than keys: rows that see nothing, with NaN in them, and
+    rows that see one key, before rows that see more."""
+    lens = [(45, 9), (70, 66)]
+    t, w = (Packed(lens, dtype, 2, 1, 64, mask=mask, prefix=prefix) for _ in range(2))
+    dead = [i for i in range(36)] if prefix is None else []
+    dead += [45 + i for i in range(4)]
+    one = [36] if prefix is None else list(range(37))
+    one += [45 + 4]
+    t.q[dead], t.d_out[dead] = math.nan, math.nan
+    a = t.args(gpu, True)
+    ops.attention(gpu, a)
+    ops.attention_backward(gpu, a, t.grads())
+    want = w.reference(True)
+    for name in ("out", "lse", "d_q", "d_k", "d_v"):
+        assert_within(getattr(t, name), *want[name], name)
+    assert torch.all(t.out[dead] == 0.0) and torch.all(t.lse[:, dead] == -math.inf)
+    assert torch.all(t.d_q[dead + one] == 0.0)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("documents,heads", [(200, 2), (4300, 1)])
+def test_many_documents(gpu, dtype, documents, heads):
+    t = Packed([(i % 4, i % 4) for i in range(documents)], dtype, heads, 1, 16, mask="causal")
+    a = t.args(gpu, True)
+    ops.attention(gpu, a)
+    ops.attention_backward(gpu, a, t.grads())
+    t.check(["out", "lse", "d_q", "d_k", "d_v"], True)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("scale", [-0.2, 0.0])
+@pytest.mark.parametrize("options", [dict(), dict(cap=7.0), dict(bias=0.1)])
+def test_scales_below_and_at_zero(gpu, dtype, scale, options):
+    t = Packed(SELF(90, 33), dtype, 2, 1, 64, mask="causal", scale=scale, **options)
+    a = t.args(gpu, True)
+    ops.attention(gpu, a)
+    ops.attention_backward(gpu, a, t.grads())
+    t.check(["out", "lse", "d_q", "d_k", "d_v", "d_slopes"], True)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("axes", [0, 1, 2, 3])
+@pytest.mark.parametrize("d", [40, 128])
+def test_few_tokens_with_a_bias_and_hidden_places(gpu, dtype, axes, d):
+    """A decoding step's chunk, whose last key its earlier rows do not see,
+    whatever that holds."""
+    lens = [(4, 500), (1, 77), (3, 130), (2, 3)]
+    t, w = (Packed(lens, dtype, 6, 3, d, mask="causal", bias=0.1, axes=axes, gap=2) for _ in range(2))
+    last = [2 + 499, 2 + 500 + 77 + 129, 2 + 500 + 77 + 130 + 2]
+    t.k[last], t.v[last] = math.nan, math.inf
+    ops.attention(gpu, t.args(gpu, False, 500))
+    want = w.reference(False)
+    clean = [2, 3, 4, 6, 7, 8, 10]  # rows 2 to 5, 6, 7 to 9 and 10 to 11, without each chunk's last
+    assert_within(t.out[clean], want["out"][0][clean], want["out"][1][clean], "out")
+    assert_within(t.lse[:, clean], want["lse"][0][:, clean], want["lse"][1][:, clean], "lse")
+    assert torch.all(t.out[:2] == 7.0) and torch.all(t.out[-2:] == 7.0)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_tensors_without_rows(gpu, dtype):
+    t = Packed([(5, 0), (3, 0)], dtype, 2, 1, 64)
+    a = t.args(gpu, True)
+    ops.attention(gpu, a)
+    ops.attention_backward(gpu, a, t.grads())
+    assert torch.all(t.out == 0.0) and torch.all(t.lse == -math.inf) and torch.all(t.d_q == 0.0)
+    t = Packed([(0, 5), (0, 130)], dtype, 2, 1, 64, mask="causal", bias=0.1)
+    a = t.args(gpu, True)
+    ops.attention(gpu, a)
+    ops.attention_backward(gpu, a, t.grads())
+    assert torch.all(t.d_k == 0.0) and torch.all(t.d_v == 0.0) and torch.all(t.d_slopes == 0.0)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("lens,d", [([(1, 3000)], 128), ([(70, 900)], 64), ([(700, 700)], 128)])
+def test_a_workspace_is_as_large_as_it_says(gpu, dtype, lens, d):
+    t = Packed(lens, dtype, 4, 2, d, mask="causal", bias=0.1)
+    a = t.args(gpu, True)
+    ops.attention(gpu, a)
+    ops.attention_backward(gpu, a, t.grads())
+    assert torch.all(t.workspace[-16:] == 0xFF)
+    n = Norm(700, 200, dtype)
+    ops.layer_norm(gpu, n.args())
+    ops.layer_norm_backward(gpu, n.args(), n.grads(gpu))
+    assert torch.all(n.workspace[-16:] == 0xFF)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_a_key_head_that_is_broadcast(gpu, dtype):
+    """Two key heads that are one tensor's, read through a head stride of
+    zero: each keeps the gradients of its own queries."""
+    t, w = (Packed(SELF(100, 57), dtype, 4, 2, 64, mask="causal") for _ in range(2))
+    for x in (w.k, w.v):
+        x[:, 1] = x[:, 0]
+    a = t.args(gpu, True)
+    a.k.head_stride = a.v.head_stride = 0
+    ops.attention(gpu, a)
+    ops.attention_backward(gpu, a, t.grads())
+    want = w.reference(True)
+    for name in ("out", "lse", "d_q", "d_k", "d_v"):
+        assert_within(getattr(t, name), *want[name], name)
+
+
+def test_two_streams_at_once(gpu):
+    """Calls that overlap in time, a workspace each, give the bits of calls in
+    turn."""
+    problems = [Packed(SELF(300, 200), "bf16", 4, 2, 128, mask="causal", cap=20.0, seed=s) for s in (1, 2)]
+    ready = [(t, t.args(gpu, True), t.grads()) for t in problems]
+    want = []
+    for t, a, g in ready:
+        ops.attention(gpu, a)
+        ops.attention_backward(gpu, a, g)
+        want.append([x.clone() for x in (t.out, t.lse, t.d_q, t.d_k, t.d_v)])
+        for x in (t.out, t.lse, t.d_q, t.d_k, t.d_v):
+            x.zero_()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    contexts = [hip.Context(0, stream=s.cuda_stream) for s in streams]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for ctx, (t, a, g) in zip(contexts, ready):
+            ops.attention(ctx, a)
+            ops.attention_backward(ctx, a, g)
+    torch.cuda.synchronize()
+    for (t, _, _), kept in zip(ready, want):
+        assert all(torch.equal(x, y) for x, y in zip((t.out, t.lse, t.d_q, t.d_k, t.d_v), kept))
+    for ctx in contexts:
+        ctx.close()
+
+
+def test_rotary_of_more_rows_than_a_grid_has_threads(gpu):
+    """One pair of a head of 256, a workgroup a row: 2^23 of them and some."""
+    rows = 2**23 + 7
+    x = torch.ones(rows, 1, 256, device="cuda", dtype=torch.float16)
+    x[:, 0, 1] = 0.0
+    positions = (torch.arange(rows, device="cuda", dtype=torch.int32) % 1000).contiguous()
+    view = ops.Heads(x.data_ptr(), 256, 256)
+    ops.rotary(gpu, ops.rotary_table([1], 10.0), ops.RotaryArgs(dtype=hip.F16, rows=rows, q_heads=1, head_dim=256, positions=positions.data_ptr(), q_in=view, q_out=view))
+    phi = positions.double()
+    # a sine of f32 in 64-bit reduced angles, rounded once
+    for c, want in ((0, phi.cos()), (1, phi.sin())):
+        assert_within(x[:, 0, c], want, half_step(torch.float16) * want.abs() + 16 * F32 + 2.0**-25, f"channel {c}")
+    assert torch.all(x[-9:, 0, 2:] == 1.0)

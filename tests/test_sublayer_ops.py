@@ -242,7 +242,7 @@ def attention_args(**changed):
 
 
 def attention_grads(**changed):
-    g = ops.AttentionGrads(d_out=ops.Heads(AT, 256, 64), d_q=ops.Heads(2 * AT, 256, 64), d_k=ops.Heads(3 * AT, 128, 64), d_v=ops.Heads(4 * AT, 128, 64))
+    g = ops.AttentionGrads(d_out=ops.Heads(AT, 256, 64), d_q=ops.Heads(5 * AT, 256, 64), d_k=ops.Heads(3 * AT, 128, 64), d_v=ops.Heads(4 * AT, 128, 64))
     for name, value in changed.items():
         setattr(g, name, value)
     return g
@@ -291,3 +291,28 @@ def test_attention_accepted(host):
     assert n.value == 128
     assert host.bl_packed_attention_workspace(ctx, C.byref(attention_args()), 2, C.byref(n)) == INVALID
     assert host.bl_packed_attention_workspace(ctx, C.byref(attention_args()), 0, None) == INVALID
+
+
+@pytest.mark.parametrize("changed,code,says", [
+    (dict(scale=3e38), INVALID, "beyond f32"), (dict(softcap=3e38), INVALID, "beyond f32"), (dict(softcap=1e-40), INVALID, "beyond f32"),
+    (dict(out=ops.Heads(AT, 256, 64)), INVALID, "out is q"), (dict(k=ops.Heads(2 * AT, 256, 64)), INVALID, "out is k"), (dict(out=ops.Heads(2 * AT, 64, 64)), INVALID, "overlap"),
+    (dict(out=ops.Heads(2 * AT, 248, 64)), INVALID, "overlap"), (dict(out=ops.Heads(2 * AT, 64, 632)), INVALID, "overlap"),
+    (dict(k_rows=2**29), LARGE, "rows"), (dict(documents=2**23), LARGE, "documents"),
+])
+def test_attention_refuses_what_it_would_write_twice_or_could_not_launch(host, changed, code, says):
+    refused(host, host.bl_packed_attention, [attention_args(**changed)], code, says)
+
+
+@pytest.mark.parametrize("more,says", [
+    (dict(d_q=ops.Heads(AT, 256, 64)), "d_q is q"), (dict(d_v=ops.Heads(3 * AT, 128, 64)), "d_v is d_k"), (dict(d_k=ops.Heads(5 * AT, 256, 64)), "d_k is d_q"),
+    (dict(d_out=ops.Heads(4 * AT, 256, 64)), "d_v is d_out"), (dict(d_q=ops.Heads(2 * AT, 256, 64)), "d_q is out"),
+])
+def test_gradients_of_attention_lie_apart(host, more, says):
+    refused(host, host.bl_packed_attention_backward, [attention_args(), attention_grads(**more)], INVALID, says)
+
+
+def test_attention_takes_heads_and_rows_in_either_order(host):
+    accepted(host, host.bl_packed_attention, [attention_args(out=ops.Heads(2 * AT, 64, 640))])
+    accepted(host, host.bl_packed_attention, [attention_args(q_rows=1, out=ops.Heads(2 * AT, 0, 64))])
+    accepted(host, host.bl_packed_attention, [attention_args(k_rows=0, k=ops.Heads(2 * AT, 0, 0))])
+    accepted(host, host.bl_packed_attention, [attention_args(softcap=1e-30)])
