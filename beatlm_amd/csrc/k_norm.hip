@@ -1,13 +1,16 @@
 // LayerNorm over strided rows and its gradients (include/beatlm_ops.h).
 //
 // Both directions read each row once: TPR threads (a quarter of a wave to
-// sixteen waves) keep it in registers, 16 values each, so the variance is the mean of squares
-// about the mean (two passes over registers, no cancellation) and nothing is
-// read twice. The bound is HBM: forward x in, y out; backward x and dy in, dx
-// out. Rows come and go in 16-byte pieces wherever they start (the memory
-// system takes them at any element's address: 4097 x 1003 f32 forward and
-// backward 26 us, an element at a time 42), their last few values one by one. What the sums do not need is loaded before them, and the backward
+// sixteen waves) keep it in registers, 16 values each, so the variance is the
+// mean of squares about the mean (two passes over registers, no cancellation)
+// and nothing is read twice. The bound is HBM: forward x in, y out; backward x
+// and dy in, dx out. Rows come and go in 16-byte pieces wherever they start
+// (the memory system takes them at any element's address; 4097 x 1003 f32
+// forward and backward: 23 us, an element at a time 43), their last few values
+// one by one. What the sums do not need is loaded before them, and the backward
 // loads its next row while it finishes the last, so one latency is paid a row.
+// 21920 x 768 bf16: forward 16.6 us, 4.1 TB/s, backward 21.0, 4.8 TB/s, and
+// 4.2 for the weights' gradients' second launch.
 //
 // The weights' gradients are sums over rows: a workgroup of the backward walks
 // rows with a stride of the grid and keeps its columns' two sums in registers;

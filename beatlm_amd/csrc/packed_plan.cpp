@@ -21,7 +21,7 @@ PackedPlan plan_packed(const bl_packed_attention_args &a, uint32_t compute_units
     // The streamed side is split where there are few workgroups, each split
     // keeping 64 streamed rows or more. The forward splits where the chip is
     // not covered once, then to four workgroups a compute unit (16 tokens over
-    // 16384 keys 71 us, two 83; packed images that cover it, 360 workgroups: 49
+    // 3449 to 16326 keys 71 us, two 83; packed images that cover it, 360 workgroups: 49
     // us unsplit, 63 in three). The backward's causal rows are longer and its
     // workgroups larger: it splits to two a unit (8192 tokens, 260 workgroups:
     // d_k and d_v 0.81 ms in two, 1.3 unsplit).
