@@ -753,3 +753,24 @@ def test_rotary_of_more_rows_than_a_grid_has_threads(gpu):
     for c, want in ((0, phi.cos()), (1, phi.sin())):
         assert_within(x[:, 0, c], want, half_step(torch.float16) * want.abs() + 16 * F32 + 2.0**-25, f"channel {c}")
     assert torch.all(x[-9:, 0, 2:] == 1.0)
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("d,keys", [(16, 60), (128, 60), (64, 1000)])
+def test_the_slopes_gradient_does_not_see_the_statistics_rounding(gpu, dtype, d, keys):
+    """Keys of one value leave the scores without gradient, whatever P is. lse
+    is about 2000 here, so rounding it to f32 scales a row's P by up to 2^-13."""
+    t = Packed([(1, keys)], dtype, 8, 2, d, bias=0.02, scale=1.0)
+    t.q[..., 0], t.k[..., 0] = 45.0, 45.0
+    t.v[:] = t.v[:1].clone()
+    a = t.args(gpu, True)
+    ops.attention(gpu, a)
+    ops.attention_backward(gpu, a, t.grads())
+    far = (keys - 1 - torch.arange(keys, device="cuda")).double()
+    for h in range(8):
+        q, k = t.q[0, h].double(), t.k[:, h // 4].double()
+        p = (k @ q - float(t.slopes[h]) * far).softmax(0)
+        dp = float((t.d_out[0, h].double().abs() * t.v[0, h // 4].double().abs()).sum())
+        # three sums of `keys` terms in f32, and a few products
+        most = (3 * keys + 16) * F32 * dp * float((p * far).sum())
+        assert abs(float(t.d_slopes[h])) <= most, (h, float(t.d_slopes[h]), most)
