@@ -56,15 +56,16 @@ struct PackedParams {
     float *stats;    // forward [splits][places][2], d_q [splits][places][4]; places = q_rows * q_heads
     // backward, [q_heads][q_rows] each
     float *delta;    // sum_j P_j dP_j of each row
-    float *largest;  // its largest |dO| (f16)
+    float *bound;    // a bound of its |dP| (f16)
     float *d_slope;  // its part of d_slopes
+    float *norms;    // [kv_heads][slots of 128 keys]: the values' largest squared norm (f16)
 };
 struct PackedPlan {
     uint32_t splits, splits_q, splits_kv;
     bool few;
     uint32_t tile_dim;  // channels of the kernels' tiles: 64 or 128
     uint64_t partial_bytes, stats_bytes;                     // forward
-    uint64_t row_bytes, back_partial_bytes, back_stats_bytes; // backward
+    uint64_t row_bytes, back_partial_bytes, back_stats_bytes, norm_bytes; // backward
     uint64_t forward_bytes, backward_bytes;
 };
 PackedPlan plan_packed(const bl_packed_attention_args &a, uint32_t compute_units);

@@ -49,7 +49,8 @@ PackedPlan plan_packed(const bl_packed_attention_args &a, uint32_t compute_units
     const uint64_t of_kv = plan.splits_kv > 1 ? plan.splits_kv * 2 * key_places * plan.tile_dim * sizeof(float) : 0;
     plan.back_partial_bytes = rounded(of_q > of_kv ? of_q : of_kv);  // one after the other
     plan.back_stats_bytes = plan.splits_q > 1 ? rounded(plan.splits_q * places * 4 * sizeof(float)) : 0;
-    plan.backward_bytes = 3 * plan.row_bytes + plan.back_partial_bytes + plan.back_stats_bytes;
+    plan.norm_bytes = a.dtype == BL_F16 ? rounded(keys_whole * sizeof(float)) : 0;
+    plan.backward_bytes = 3 * plan.row_bytes + plan.back_partial_bytes + plan.back_stats_bytes + plan.norm_bytes;
     return plan;
 }
 
@@ -72,10 +73,11 @@ hipError_t launch_packed_backward(const PackedParams &q, const PackedPlan &plan,
     p.splits_q = plan.splits_q;
     p.splits_kv = plan.splits_kv;
     p.delta = (float *)at;
-    p.largest = (float *)(at + plan.row_bytes);
+    p.bound = (float *)(at + plan.row_bytes);
     p.d_slope = (float *)(at + 2 * plan.row_bytes);
     p.partial = (float *)(at + 3 * plan.row_bytes);
     p.stats = (float *)(at + 3 * plan.row_bytes + plan.back_partial_bytes);
+    p.norms = (float *)(at + 3 * plan.row_bytes + plan.back_partial_bytes + plan.back_stats_bytes);
     switch (p.a.dtype) {
     case BL_F32: return packed_backward<float>(p, plan, s);
     case BL_F16: return packed_backward<_Float16>(p, plan, s);
