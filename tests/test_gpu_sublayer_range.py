@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from beatlm_amd import hip, ops
-from tests.opsdata import Packed
+from tests.opsdata import F32, Packed, assert_within, half_step
 
 pytestmark = pytest.mark.gpu
 
@@ -56,3 +56,35 @@ def test_gradients_under_large_values(gpu, dtype, d, mask):
     ops.attention(gpu, a)
     ops.attention_backward(gpu, a, t.grads())
     t.check(["out", "lse", "d_q", "d_k", "d_v"], True)
+
+
+# Flat rows over so many keys that each probability is 100.5 of f16's smallest steps
+LONG = 166937
+# what f32 may put on a sum over them: at most 1024 splits, joined in turn, of at most 192 keys
+SUMS = F32 * (1024 + 192 + 64)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_gradients_of_long_flat_rows_keep_their_digits(gpu, dtype, d):
+    t = Packed([(3, LONG)], dtype, 1, 1, d)
+    t.q.zero_()
+    t.q[..., 0] = 1.0
+    t.k[..., 0] = 0.0
+    t.d_out *= 1000.0
+    a = t.args(gpu, True)
+    ops.attention(gpu, a)
+    ops.attention_backward(gpu, a, t.grads())
+    u, p, scale = half_step(t.torch_dtype), 1.0 / LONG, d**-0.5
+    q, k, v, g = (x[:, 0].double() for x in (t.q, t.k, t.v, t.d_out))
+    # P once rounded for the products, the output once
+    want = p * g.sum(0).expand(LONG, d)
+    assert_within(t.d_v[:, 0], want, u * want.abs() + (u + SUMS) * p * g.abs().sum(0), "d_v")
+    dp, size = g @ v.T, g.abs() @ v.abs().T
+    ds = p * (dp - dp.mean(1, keepdim=True))
+    # dS is off by its own rounding and by its sums', and by f16's smallest step, 2^-25, of 2^-10 of
+    # twice a bound of |dP|
+    bound = 2 * g.norm(dim=1, keepdim=True) * v.norm(dim=1).max()
+    off = u * ds.abs() + p * SUMS * (size + size.mean(1, keepdim=True)) + (2.0**-35 * bound if dtype == "f16" else 0.0)
+    want = scale * ds.T @ q
+    assert_within(t.d_k[:, 0], want, u * want.abs() + scale * off.T @ q.abs() + 2.0**-25, "d_k")
