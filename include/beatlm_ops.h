@@ -171,7 +171,8 @@ int bl_rotary(bl_ctx *ctx, const bl_rotary_table *table, const bl_rotary_args *a
  * scores count as exactly -inf whatever q and k hold there; a hidden key's v
  * may be anything too. Sums, statistics and scores are f32; for the matrix
  * cores the probabilities, and the scores' gradients, are rounded to the
- * tensors' type (f32 stays f32). What a call writes overlaps nothing else.
+ * tensors' type (f32 stays f32; f16 holds them times powers of two that keep
+ * them in its range). What a call writes overlaps nothing else.
  *
  * The offsets are device arrays, read when the kernels run (a captured graph
  * may be replayed with others); they are clamped to the tensors' rows, so

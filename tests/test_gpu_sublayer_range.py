@@ -88,3 +88,30 @@ def test_gradients_of_long_flat_rows_keep_their_digits(gpu, dtype, d):
     off = u * ds.abs() + p * SUMS * (size + size.mean(1, keepdim=True)) + (2.0**-35 * bound if dtype == "f16" else 0.0)
     want = scale * ds.T @ q
     assert_within(t.d_k[:, 0], want, u * want.abs() + scale * off.T @ q.abs() + 2.0**-25, "d_k")
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_a_long_tail_of_small_probabilities_keeps_its_digits(gpu, dtype):
+    """One key ahead of all others, which have half the weight together: each is
+    101.48 of f16's smallest steps beside the first. 256 heads on one key head's
+    tensors, so that no split takes the tail apart."""
+    heads, d = 256, 64
+    t = Packed([(1, LONG)], dtype, heads, 1, d, scale=1.0)
+    t.q.zero_()
+    t.q[..., 0] = 1.0
+    t.k.zero_()
+    t.k[0, 0, 0] = 12.015625
+    t.v[:], t.v[0] = 1.0, 0.0
+    a = t.args(gpu, False)
+    a.kv_heads = heads
+    a.k.head_stride = a.v.head_stride = 0
+    n = ops.attention_workspace(gpu, a)
+    workspace = torch.empty(n + 16, device="cuda", dtype=torch.uint8)
+    a.workspace, a.workspace_bytes = workspace.data_ptr(), n
+    ops.attention(gpu, a)
+    u = half_step(t.torch_dtype)
+    first = float(t.k[0, 0, 0].double())
+    tail = (LONG - 1) * torch.tensor(-first, dtype=torch.float64).exp().item()
+    want = torch.full_like(t.out, tail / (1 + tail), dtype=torch.float64)
+    # P once rounded, the output once; unsplit sums of equal terms in f32, a lane's 32 of 64 keys a tile
+    assert_within(t.out, want, want * (2 * u + F32 * (LONG / 2 + 64)), "out")
