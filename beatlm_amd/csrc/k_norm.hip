@@ -170,8 +170,8 @@ __global__ __launch_bounds__(norm_threads<TPR>) void norm_backward_kernel(NormPa
         for (int n = 0; n < N; n++)
 #pragma unroll
             for (int e = 0; e < VEC; e++) {
-                // dy is 0 beyond the row, whatever n is there
-                n_[n][e] = ((float)x.v[n][e] - mean) * rstd;
+                // dy is 0 beyond the row; n has to be finite there, as mean * rstd need not be
+                n_[n][e] = P::col(lane, n) + e < p.cols ? ((float)x.v[n][e] - mean) * rstd : 0.0f;
                 d[n][e] = (float)dy.v[n][e];
                 dg[n][e] += d[n][e] * n_[n][e];
                 db[n][e] += d[n][e];

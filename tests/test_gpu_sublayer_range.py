@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from beatlm_amd import hip, ops
-from tests.opsdata import F32, Packed, assert_within, half_step
+from tests.opsdata import DTYPES, F32, Packed, assert_within, half_step
 
 pytestmark = pytest.mark.gpu
 
@@ -115,3 +115,30 @@ def test_a_long_tail_of_small_probabilities_keeps_its_digits(gpu, dtype):
     want = torch.full_like(t.out, tail / (1 + tail), dtype=torch.float64)
     # P once rounded, the output once; unsplit sums of equal terms in f32, a lane's 32 of 64 keys a tile
     assert_within(t.out, want, want * (2 * u + F32 * (LONG / 2 + 64)), "out")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("cols", [5, 200, 1003, 4099])
+def test_layer_norm_s_gradients_of_flat_rows_of_large_values(gpu, dtype, cols):
+    """x is its mean everywhere, so n is 0, and mean times rstd is beyond f32."""
+    torch_dtype, code = DTYPES[dtype]
+    rows, epsilon = 3, 1e-6
+    g = torch.Generator(device="cuda").manual_seed(cols)
+    make = lambda *s: torch.randn(*s, generator=g, device="cuda").to(torch_dtype)  # noqa: E731
+    x = torch.full((rows, cols), 2.0**121, device="cuda", dtype=torch_dtype)
+    dy, gamma, dx = make(rows, cols), make(cols), torch.empty_like(x)
+    mean, rstd = torch.full((rows,), 2.0**121, device="cuda"), torch.full((rows,), epsilon**-0.5, device="cuda")
+    d_gamma, d_beta = (torch.empty(cols, device="cuda") for _ in range(2))
+    a = ops.LayerNormArgs(dtype=code, rows=rows, cols=cols, epsilon=epsilon, x_stride=cols, x=x.data_ptr(), gamma=gamma.data_ptr(),
+                          mean=mean.data_ptr(), rstd=rstd.data_ptr())
+    n = ops.layer_norm_backward_workspace(gpu, a)
+    workspace = torch.empty(n, device="cuda", dtype=torch.uint8)
+    ops.layer_norm_backward(gpu, a, ops.LayerNormGrads(dy=dy.data_ptr(), dy_stride=cols, dx=dx.data_ptr(), dx_stride=cols, d_gamma=d_gamma.data_ptr(),
+                                                       d_beta=d_beta.data_ptr(), workspace=workspace.data_ptr(), workspace_bytes=n))
+    scaled, r = dy.double() * gamma.double(), rstd.double()[:, None]
+    want = r * (scaled - scaled.mean(1, keepdim=True))
+    # a sum of 16 values a thread and at most 22 additions of those, one product and one difference each
+    off = r * F32 * (40 * scaled.abs().mean(1, keepdim=True) + 4 * scaled.abs())
+    assert_within(dx, want, half_step(torch_dtype) * want.abs() + off, "dx")
+    assert torch.all(d_gamma == 0.0)
+    assert_within(d_beta, dy.double().sum(0), F32 * (rows + 8) * dy.double().abs().sum(0), "d_beta")
