@@ -265,28 +265,26 @@ uint32_t threads_per_row(uint32_t cols) { return cols <= 16 * EPT ? 16 : cols <=
 template <typename T>
 hipError_t forward(const NormParams &p, hipStream_t s) {
     switch (threads_per_row(p.cols)) {
-    case 16: norm_forward_kernel<T, 16><<<p.groups, 256, 0, s>>>(p); break;
-    case 64: norm_forward_kernel<T, 64><<<p.groups, 256, 0, s>>>(p); break;
-    case 256: norm_forward_kernel<T, 256><<<p.groups, 256, 0, s>>>(p); break;
-    default: norm_forward_kernel<T, 1024><<<p.groups, 1024, 0, s>>>(p); break;
+    case 16: return run_kernel(norm_forward_kernel<T, 16>, p.groups, 256, s, p);
+    case 64: return run_kernel(norm_forward_kernel<T, 64>, p.groups, 256, s, p);
+    case 256: return run_kernel(norm_forward_kernel<T, 256>, p.groups, 256, s, p);
+    default: return run_kernel(norm_forward_kernel<T, 1024>, p.groups, 1024, s, p);
     }
-    return hipGetLastError();
 }
 
 template <typename T>
 hipError_t backward(const NormParams &p, hipStream_t s) {
     if (p.groups) {
+        hipError_t e;
         switch (threads_per_row(p.cols)) {
-        case 16: norm_backward_kernel<T, 16><<<p.groups, 256, 0, s>>>(p); break;
-        case 64: norm_backward_kernel<T, 64><<<p.groups, 256, 0, s>>>(p); break;
-        case 256: norm_backward_kernel<T, 256><<<p.groups, 256, 0, s>>>(p); break;
-        default: norm_backward_kernel<T, 1024><<<p.groups, 1024, 0, s>>>(p); break;
+        case 16: e = run_kernel(norm_backward_kernel<T, 16>, p.groups, 256, s, p); break;
+        case 64: e = run_kernel(norm_backward_kernel<T, 64>, p.groups, 256, s, p); break;
+        case 256: e = run_kernel(norm_backward_kernel<T, 256>, p.groups, 256, s, p); break;
+        default: e = run_kernel(norm_backward_kernel<T, 1024>, p.groups, 1024, s, p); break;
         }
-        const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
-    norm_reduce_kernel<<<(2 * p.cols + 15) / 16, 1024, 0, s>>>(p);
-    return hipGetLastError();
+    return run_kernel(norm_reduce_kernel, (2 * p.cols + 15) / 16, 1024, s, p);
 }
 
 }  // namespace

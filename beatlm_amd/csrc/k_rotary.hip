@@ -109,8 +109,8 @@ hipError_t launch(const RotaryParams &p, uint32_t compute_units, hipStream_t s) 
     const uint64_t most = 1u << 23, groups = ((uint64_t)p.rows + g.rows - 1) / g.rows;
     for (uint64_t done = 0; done < groups; done += most) {
         g.first = (uint32_t)(done * g.rows);
-        rotary_kernel<T, VEC><<<(uint32_t)(groups - done < most ? groups - done : most), 256, 0, s>>>(p, g);
-        if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+        const uint32_t grid = (uint32_t)(groups - done < most ? groups - done : most);
+        if (const hipError_t e = run_kernel(rotary_kernel<T, VEC>, grid, 256, s, p, g); e != hipSuccess) return e;
     }
     return hipSuccess;
 }

@@ -1,4 +1,4 @@
-// Device helpers the packed sublayer's kernels share: 16-byte chunks of the
+// What the packed sublayer's kernels share: their launch, 16-byte chunks of the
 // three element types as f32 values, and their rounding back (to nearest even,
 // once, at the store).
 #pragma once
@@ -7,6 +7,14 @@
 #include "ops.hpp"
 
 namespace bl {
+
+// Launches a kernel and returns that launch's own status: the thread's last
+// error may be the host's, from before the call.
+template <typename... P>
+hipError_t run_kernel(void (*kernel)(P...), dim3 grid, uint32_t threads, hipStream_t s, const P &...params) {
+    void *args[] = {(void *)&params...};
+    return hipLaunchKernel((const void *)kernel, grid, dim3(threads), args, 0, s);
+}
 
 // VEC elements at p (16-byte aligned when VEC > 1) as f32.
 template <typename T, int VEC>

@@ -1,0 +1,113 @@
+"""What the packed sublayer's operators make of the HIP runtime's answers: the
+built library, over a stand-in for the runtime's calls that knows two devices
+and fails where a test says so. No GPU."""
+
+import pathlib
+import subprocess
+import sys
+
+import pytest
+
+ROOT = pathlib.Path(__file__).resolve().parent.parent
+
+STAND_IN = r"""
+#include <hip/hip_runtime_api.h>
+#include <string.h>
+extern "C" {
+int launches = 0, failing = -1, current = 0, refused_streams = 0;
+hipError_t pending = hipSuccess;  // the host thread's last error
+static hipError_t failed(hipError_t e) { return pending = e; }
+hipError_t hipGetLastError(void) { const hipError_t e = pending; pending = hipSuccess; return e; }
+hipError_t hipPeekAtLastError(void) { return pending; }
+hipError_t hipGetDeviceCount(int *n) { *n = 2; return hipSuccess; }
+hipError_t hipGetDevice(int *d) { *d = current; return hipSuccess; }
+hipError_t hipSetDevice(int d) { if (d < 0 || d > 1) return failed(hipErrorInvalidDevice); current = d; return hipSuccess; }
+hipError_t hipGetDeviceProperties(hipDeviceProp_t *p, int) { memset(p, 0, sizeof *p); p->multiProcessorCount = 256; p->warpSize = 64; return hipSuccess; }
+hipError_t hipDeviceGetAttribute(int *v, hipDeviceAttribute_t, int) { *v = 100000; return hipSuccess; }
+// A stream's address is its device's number times 16, and 16; others are no streams.
+hipError_t hipStreamGetDevice(hipStream_t s, hipDevice_t *d) {
+    if ((size_t)s != 16 && (size_t)s != 32) return failed(hipErrorInvalidHandle);
+    *d = (int)((size_t)s / 16) - 1;
+    return hipSuccess;
+}
+hipError_t hipLaunchKernel(const void *, dim3, dim3, void **, size_t, hipStream_t) {
+    return launches++ == failing ? failed(hipErrorOutOfMemory) : hipSuccess;
+}
+}
+"""
+
+PROGRAM = r"""
+import ctypes as C
+import sys
+stand_in = C.CDLL(sys.argv[1], mode=C.RTLD_GLOBAL)  # before the library, whose calls it answers
+sys.path.insert(0, sys.argv[2])
+from beatlm_amd import hip, ops
+launches, failing, current, pending = (C.c_int.in_dll(stand_in, n) for n in ("launches", "failing", "current", "pending"))
+AT = 1 << 40  # addresses that nothing looks at
+view = lambda at, stride: ops.Heads(at * AT, stride, 64)
+
+norm = ops.LayerNormArgs(dtype=hip.F16, rows=4, cols=20, epsilon=1e-6, x_stride=20, y_stride=20, x=AT, gamma=2 * AT, beta=3 * AT, y=4 * AT, mean=5 * AT, rstd=6 * AT)
+norm_grads = ops.LayerNormGrads(dy=7 * AT, dy_stride=20, dx=8 * AT, dx_stride=20, d_gamma=9 * AT, d_beta=10 * AT, workspace=11 * AT, workspace_bytes=1 << 30)
+turn = ops.RotaryArgs(dtype=hip.F32, rows=9, q_heads=4, k_heads=2, head_dim=64, positions=AT, q_in=view(2, 256), q_out=view(3, 256), k_in=view(4, 128), k_out=view(5, 128))
+table = ops.rotary_table([16], 100.0)
+def attention(dtype, rows):
+    return ops.AttentionArgs(dtype=dtype, q_heads=4, kv_heads=2, head_dim=64, q_rows=rows, k_rows=rows, documents=1, scale=0.125, slopes=AT, q=view(2, 256), k=view(3, 128),
+                             v=view(4, 128), out=view(5, 256), lse=6 * AT, workspace=7 * AT, workspace_bytes=1 << 34)
+grads = ops.AttentionGrads(d_out=view(8, 256), d_q=view(9, 256), d_k=view(10, 128), d_v=view(11, 128), d_slopes=12 * AT)
+CALLS = {  # name: (the call, its launches)
+    "norm": (lambda c: ops.layer_norm(c, norm), 1),
+    "norm backward": (lambda c: ops.layer_norm_backward(c, norm, norm_grads), 2),
+    "rotary": (lambda c: ops.rotary(c, table, turn), 1),
+    "attention": (lambda c: ops.attention(c, attention(ops.BF16, 128 * 256)), 1),
+    "attention split": (lambda c: ops.attention(c, attention(hip.F32, 300)), 2),
+    "backward": (lambda c: ops.attention_backward(c, attention(ops.BF16, 128 * 512), grads), 3),
+    "backward split": (lambda c: ops.attention_backward(c, attention(ops.BF16, 300), grads), 5),
+    "backward f16": (lambda c: ops.attention_backward(c, attention(hip.F16, 128 * 512), grads), 4),
+    "backward f32": (lambda c: ops.attention_backward(c, attention(hip.F32, 300), grads), 5),
+}
+exec(sys.stdin.read())
+"""
+
+
+@pytest.fixture(scope="module")
+def run(tmp_path_factory):
+    d = tmp_path_factory.mktemp("errors")
+    (d / "stand_in.cpp").write_text(STAND_IN)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-shared", "-fPIC", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", str(d / "stand_in.cpp"),
+                    "-o", str(d / "libstandin.so"), "-w"], check=True)
+    (d / "program.py").write_text(PROGRAM)
+
+    def program(text):
+        r = subprocess.run([sys.executable, str(d / "program.py"), str(d / "libstandin.so"), str(ROOT)], input=text, capture_output=True, text=True)
+        assert r.returncode == 0, r.stderr
+
+    return program
+
+
+def test_a_host_s_earlier_error_is_not_the_call_s(run):
+    """An error of the host's own, not yet asked for: the calls succeed, launch
+    all their kernels and leave it to the host."""
+    run("""
+c = hip.Context(0, stream=16)
+for name, (call, expected) in CALLS.items():
+    launches.value, pending.value = 0, 101
+    call(c)
+    assert (launches.value, pending.value) == (expected, 101), (name, launches.value, expected, pending.value)
+""")
+
+
+def test_a_launch_that_fails_is_the_call_s(run):
+    """Whichever of a call's launches fails, the call says so and launches no
+    more after it."""
+    run("""
+c = hip.Context(0, stream=16)
+for name, (call, expected) in CALLS.items():
+    for n in range(expected):
+        launches.value, failing.value = 0, n
+        try:
+            call(c)
+        except hip.BackendError as e:
+            assert e.code == hip.ERR_HIP and launches.value == n + 1, (name, n, e, launches.value)
+        else:
+            raise AssertionError((name, n))
+""")
