@@ -112,7 +112,9 @@ static int ctx_create(int device_ordinal, bool owns_stream, hipStream_t stream, 
     // Messages are formatted into 512 bytes: with this capacity, setting one
     // allocates nothing (the allocation-free entry point reports through it).
     ctx->error.reserve(512);
-    if ((e = hipSetDevice(device_ordinal)) != hipSuccess) { delete ctx; return BL_ERR_HIP; }
+    // The device is made current for the context's own stream alone; over a
+    // host's, the host's current device stays.
+    if (owns_stream && (e = hipSetDevice(device_ordinal)) != hipSuccess) { delete ctx; return BL_ERR_HIP; }
     hipDeviceProp_t prop;
     if ((e = hipGetDeviceProperties(&prop, device_ordinal)) != hipSuccess) { delete ctx; return BL_ERR_HIP; }
     // One stream at the default priority; the frame loop's work is ordered on it.
@@ -168,10 +170,12 @@ extern "C" int bl_ctx_create_on(int device_ordinal, void *stream, bl_ctx **out) 
 }
 
 static void ctx_free(bl_ctx *ctx) {
-    hipSetDevice(ctx->device);
-    if (ctx->owns_stream && ctx->stream) {
-        hipStreamSynchronize(ctx->stream);
-        hipStreamDestroy(ctx->stream);
+    if (ctx->owns_stream) {
+        hipSetDevice(ctx->device);
+        if (ctx->stream) {
+            hipStreamSynchronize(ctx->stream);
+            hipStreamDestroy(ctx->stream);
+        }
     }
     delete ctx;
 }

@@ -111,3 +111,20 @@ for name, (call, expected) in CALLS.items():
         else:
             raise AssertionError((name, n))
 """)
+
+
+def test_a_context_over_a_host_s_stream_leaves_the_current_device(run):
+    run("""
+for mine in (0, 1):
+    current.value = mine
+    for device in (0, 1):
+        c = hip.Context(device, stream=16 * (device + 1))
+        assert current.value == mine, (mine, device, "made")
+        ops.layer_norm(c, norm)
+        assert current.value == mine, (mine, device, "used")
+        c.close()
+        assert current.value == mine, (mine, device, "closed")
+        c = hip.Context(device, stream=0)  # the device's default stream
+        c.close()
+        assert current.value == mine, (mine, device, "default stream")
+""")
