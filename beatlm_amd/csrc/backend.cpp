@@ -163,7 +163,10 @@ extern "C" int bl_ctx_create_on(int device_ordinal, void *stream, bl_ctx **out) 
     *out = nullptr;
     if (stream) {
         hipDevice_t device = -1;
-        if (hipStreamGetDevice((hipStream_t)stream, &device) != hipSuccess) return BL_ERR_INVALID_ARGUMENT;
+        if (hipStreamGetDevice((hipStream_t)stream, &device) != hipSuccess) {
+            hipGetLastError();  // answered by this call's status: not left for the host to find
+            return BL_ERR_INVALID_ARGUMENT;
+        }
         if (device != device_ordinal) return BL_ERR_INVALID_ARGUMENT;
     }
     return ctx_create(device_ordinal, false, (hipStream_t)stream, out);

@@ -128,3 +128,16 @@ for mine in (0, 1):
         c.close()
         assert current.value == mine, (mine, device, "default stream")
 """)
+
+
+def test_a_refused_stream_leaves_no_error_behind(run):
+    run("""
+for stream in (32, 48):  # another device's, and none
+    try:
+        hip.Context(0, stream=stream)
+    except hip.BackendError as e:
+        assert e.code == hip.ERR_INVALID_ARGUMENT
+    else:
+        raise AssertionError(stream)
+    assert (pending.value, current.value) == (0, 0), stream
+""")
