@@ -28,6 +28,90 @@ int launched(bl_ctx *ctx, hipError_t e, const char *what) {
     return e == hipSuccess ? BL_OK : refuse(ctx, BL_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
 }
 
+// ---- what a call writes lies apart ----
+
+// The bytes of a strided tensor: `rows` by `heads` pieces of `width`, steps in bytes.
+struct Bytes {
+    uint64_t at, row, rows, head, heads, width;
+};
+typedef __int128 wide;  // products of a call's strides and counts
+
+Bytes bytes_of(const bl_heads &h, uint64_t rows, uint64_t heads, uint64_t head_dim, uint64_t size) {
+    return {(uint64_t)h.data, h.row_stride * size, rows, h.head_stride * size, heads, head_dim * size};
+}
+
+// The least n >= 0 with n * step mod m in [lo, hi] (0 < lo <= hi < m), or -1.
+wide first_within(wide step, wide m, wide lo, wide hi) {
+    if (step == 0) return -1;
+    if (2 * step > m) return first_within(m - step, m, m - hi, m - lo);  // counted downwards
+    const wide n = (lo + step - 1) / step;
+    if (n * step <= hi) return n;
+    // No multiple of step in [lo, hi]: so many times round m that one comes to lie in it.
+    const wide round = first_within((step - m % step) % step, step, lo % step, hi % step);
+    return round < 0 ? -1 : (lo + m * round + step - 1) / step;
+}
+
+// Whether two rows of pieces meet: from + x p of width w and y q of width v,
+// x < n, y < k.
+bool rows_meet(wide from, wide p, wide n, wide w, wide q, wide k, wide v) {
+    if (p == 0) n = 1;
+    if (q == 0) k = 1;
+    if (k == 1) q = n * p + w + v + (from < 0 ? -from : from);  // any step beyond the rest
+    // A y serves where y q lies in [t - room, t], t = from + x p + w - 1.
+    const wide t0 = from + w - 1, room = w + v - 2;
+    const wide most = (k - 1) * q + room - t0;  // x p is no more than this, and t no less than 0
+    if (most < 0 || (p == 0 && t0 < 0)) return false;
+    const wide first = t0 >= 0 ? 0 : (-t0 + p - 1) / p, last = p == 0 ? 0 : most / p < n - 1 ? most / p : n - 1;
+    if (first > last) return false;
+    if (room >= q - 1) return true;
+    const wide at = (t0 + first * p) % q;
+    if (at <= room) return true;
+    const wide steps = first_within(p % q, q, q - at, q - at + room);
+    return steps >= 0 && steps <= last - first;
+}
+
+bool overlap(Bytes a, Bytes b) {
+    for (Bytes *t : {&a, &b}) {
+        if (t->rows == 0 || t->heads == 0) return false;
+        if (t->head == 0) t->heads = 1;
+        if (t->row == 0) t->rows = 1;
+        // Pieces that lie end to end are one.
+        if (t->heads > 1 && t->head == t->width) t->width *= t->heads, t->heads = 1;
+        if (t->rows > 1 && t->row == t->width) t->width *= t->rows, t->rows = 1;
+        if (t->heads > 1 && t->head == t->width) t->width *= t->heads, t->heads = 1;
+    }
+    const auto end = [](const Bytes &t) { return (wide)t.at + (wide)t.row * (t.rows - 1) + (wide)t.head * (t.heads - 1) + t.width; };
+    if (end(a) <= (wide)b.at || end(b) <= (wide)a.at) return false;
+    // As a rule all heads of a row lie beside all of the other's: one look at
+    // them as one piece.
+    const auto all = [](const Bytes &t) { return (wide)t.head * (t.heads - 1) + t.width; };
+    if (!rows_meet((wide)a.at - (wide)b.at, a.row, a.rows, all(a), b.row, b.rows, all(b))) return false;
+    const auto meet = [&](wide heads_apart) {
+        return rows_meet((wide)a.at - (wide)b.at + heads_apart, a.row, a.rows, a.width, b.row, b.rows, b.width);
+    };
+    if (a.heads == 1 || b.heads == 1 || a.head == b.head) {  // heads by their difference alone
+        const wide step = a.heads == 1 ? b.head : a.head;
+        for (wide d = 1 - (wide)b.heads; d < (wide)a.heads; d++)
+            if (meet(d * step)) return true;
+        return false;
+    }
+    if (a.heads * b.heads > 1u << 20) return true;  // too many pairs to look at, of rows that do meet
+    for (wide x = 0; x < (wide)a.heads; x++)
+        for (wide y = 0; y < (wide)b.heads; y++)
+            if (meet(x * a.head - y * (wide)b.head)) return true;
+    return false;
+}
+
+struct Named {
+    Bytes bytes;
+    const char *name;
+};
+int check_apart(bl_ctx *ctx, const char *what, const Named &written, const Named &other) {
+    if (!overlap(written.bytes, other.bytes)) return BL_OK;
+    const bool same = written.bytes.at == other.bytes.at;
+    return refuse(ctx, BL_ERR_INVALID_ARGUMENT, "%s: %s %s %s", what, written.name, same ? "is" : "overlaps", other.name);
+}
+
 // ---- LayerNorm ----
 
 int check_norm(bl_ctx *ctx, const bl_layer_norm_args *a, const char *what) {
@@ -55,6 +139,11 @@ int check_vector(bl_ctx *ctx, const void *p, uint64_t size, const char *what, co
     if (!aligned(p, size)) return refuse(ctx, BL_ERR_INVALID_ARGUMENT, "%s: %s is misaligned", what, name);
     return BL_OK;
 }
+
+Named rows_named(const bl_layer_norm_args *a, const void *p, uint64_t stride, const char *name) {
+    return {bytes_of({(void *)p, stride, 0}, a->rows, 1, a->cols, element_size(a->dtype)), name};
+}
+Named vector_named(const bl_layer_norm_args *a, const void *p, const char *name) { return {bytes_of({(void *)p, 0, 0}, 1, 1, a->cols, element_size(a->dtype)), name}; }
 
 uint64_t norm_workspace(bl_ctx *ctx, const bl_layer_norm_args *a) {
     return (uint64_t)bl::norm_groups(a->rows, a->cols, bl_compute_units_of(ctx), bl::NORM_BACKWARD_GROUPS) * 2 * a->cols * sizeof(float);
@@ -119,23 +208,19 @@ int check_attention(bl_ctx *ctx, const bl_packed_attention_args *a, const char *
     return BL_OK;
 }
 
-// A tensor that a call writes starts where none of the others does.
-struct Named {
-    const bl_heads &h;
-    uint32_t rows;
-    const char *name;
-};
+// Tensors that a call writes share nothing with each other or with those it reads.
 template <size_t N, size_t M>
 int check_separate(bl_ctx *ctx, const char *what, const Named (&written)[N], const Named (&read)[M]) {
-    for (size_t i = 0; i < N; i++) {
-        const Named &w = written[i];
-        for (size_t j = 0; j < i + M; j++) {
-            const Named &r = j < i ? written[j] : read[j - i];
-            if (w.rows && r.rows && w.h.data == r.h.data)
-                return refuse(ctx, BL_ERR_INVALID_ARGUMENT, "%s: %s is %s", what, w.name, r.name);
-        }
-    }
+    for (size_t i = 0; i < N; i++)
+        for (size_t j = 0; j < i + M; j++)
+            if (int rc = check_apart(ctx, what, written[i], j < i ? written[j] : read[j - i])) return rc;
     return BL_OK;
+}
+Named q_named(const bl_packed_attention_args *a, const bl_heads &h, const char *name) {
+    return {bytes_of(h, a->q_rows, a->q_heads, a->head_dim, element_size(a->dtype)), name};
+}
+Named k_named(const bl_packed_attention_args *a, const bl_heads &h, const char *name) {
+    return {bytes_of(h, a->k_rows, a->kv_heads, a->head_dim, element_size(a->dtype)), name};
 }
 
 // What the kernels will read, beyond the sizes.
@@ -183,6 +268,11 @@ extern "C" int bl_layer_norm(bl_ctx *ctx, const bl_layer_norm_args *a) {
     if (!aligned(a->mean, 4) || !aligned(a->rstd, 4)) return refuse(ctx, BL_ERR_INVALID_ARGUMENT, "%s: the statistics are misaligned", what);
     if (a->x == a->y && a->x_stride != a->y_stride && a->rows > 1)
         return refuse(ctx, BL_ERR_INVALID_ARGUMENT, "%s: y is x with another stride", what);
+    const Named y = rows_named(a, a->y, a->y_stride, "y");
+    if (a->x != a->y)
+        if (int rc = check_apart(ctx, what, y, rows_named(a, a->x, a->x_stride, "x"))) return rc;
+    if (int rc = check_apart(ctx, what, y, vector_named(a, a->gamma, "gamma"))) return rc;
+    if (int rc = check_apart(ctx, what, y, vector_named(a, a->beta, "beta"))) return rc;
     if (a->rows == 0) return BL_OK;
     bl::NormParams p{};
     p.x = a->x;
@@ -228,6 +318,12 @@ extern "C" int bl_layer_norm_backward(bl_ctx *ctx, const bl_layer_norm_args *a, 
     }
     if (a->rows > 1 && ((g->dx == a->x && g->dx_stride != a->x_stride) || (g->dx == g->dy && g->dx_stride != g->dy_stride)))
         return refuse(ctx, BL_ERR_INVALID_ARGUMENT, "%s: dx is x or dy with another stride", what);
+    const Named dx = rows_named(a, g->dx, g->dx_stride, "dx");
+    if (g->dx != a->x)
+        if (int rc = check_apart(ctx, what, dx, rows_named(a, a->x, a->x_stride, "x"))) return rc;
+    if (g->dx != g->dy)
+        if (int rc = check_apart(ctx, what, dx, rows_named(a, g->dy, g->dy_stride, "dy"))) return rc;
+    if (int rc = check_apart(ctx, what, dx, vector_named(a, a->gamma, "gamma"))) return rc;
     const uint64_t need = norm_workspace(ctx, a);
     if (g->workspace_bytes < need)
         return refuse(ctx, BL_ERR_TOO_LARGE, "%s: a workspace of %llu bytes, %llu are needed", what, (unsigned long long)g->workspace_bytes,
@@ -307,6 +403,18 @@ extern "C" int bl_rotary(bl_ctx *ctx, const bl_rotary_table *t, const bl_rotary_
     if (int rc = heads(a->q_out, a->rows, a->q_heads, true, "q_out")) return rc;
     if (int rc = heads(a->k_in, a->rows, a->k_heads, false, "k_in")) return rc;
     if (int rc = heads(a->k_out, a->rows, a->k_heads, true, "k_out")) return rc;
+    const auto named = [&](const bl_heads &h, uint32_t n, const char *name) { return Named{bytes_of(h, a->rows, n, a->head_dim, size), name}; };
+    const Named q_in = named(a->q_in, a->q_heads, "q_in"), q_out = named(a->q_out, a->q_heads, "q_out");
+    const Named k_in = named(a->k_in, a->k_heads, "k_in"), k_out = named(a->k_out, a->k_heads, "k_out");
+    if (int rc = check_apart(ctx, what, k_out, q_out)) return rc;
+    if (!same(a->q_in, a->q_out))
+        if (int rc = check_apart(ctx, what, q_out, q_in)) return rc;
+    if (!same(a->k_in, a->k_out))
+        if (int rc = check_apart(ctx, what, k_out, k_in)) return rc;
+    if (a->q_in.data != a->k_in.data) {  // one input given as both is the host's to order
+        if (int rc = check_apart(ctx, what, q_out, k_in)) return rc;
+        if (int rc = check_apart(ctx, what, k_out, q_in)) return rc;
+    }
     if (a->rows == 0) return BL_OK;
     bl::RotaryParams p{};
     p.table = *t;
@@ -349,7 +457,7 @@ extern "C" int bl_packed_attention(bl_ctx *ctx, const bl_packed_attention_args *
     if (!ctx) return BL_ERR_INVALID_ARGUMENT;
     if (int rc = check_attention(ctx, a, what)) return rc;
     if (int rc = check_attention_arrays(ctx, a, what)) return rc;
-    const Named out[] = {{a->out, a->q_rows, "out"}}, in[] = {{a->q, a->q_rows, "q"}, {a->k, a->k_rows, "k"}, {a->v, a->k_rows, "v"}};
+    const Named out[] = {q_named(a, a->out, "out")}, in[] = {q_named(a, a->q, "q"), k_named(a, a->k, "k"), k_named(a, a->v, "v")};
     if (int rc = check_separate(ctx, what, out, in)) return rc;
     const bl::PackedPlan plan = bl::plan_packed(*a, bl_compute_units_of(ctx));
     if (int rc = check_workspace(ctx, a, plan.forward_bytes, what)) return rc;
@@ -377,8 +485,8 @@ extern "C" int bl_packed_attention_backward(bl_ctx *ctx, const bl_packed_attenti
     if (int rc = heads(g->d_q, a->q_rows, a->q_heads, true, "d_q")) return rc;
     if (int rc = heads(g->d_k, a->k_rows, a->kv_heads, true, "d_k")) return rc;
     if (int rc = heads(g->d_v, a->k_rows, a->kv_heads, true, "d_v")) return rc;
-    const Named grads[] = {{g->d_q, a->q_rows, "d_q"}, {g->d_k, a->k_rows, "d_k"}, {g->d_v, a->k_rows, "d_v"}};
-    const Named in[] = {{a->q, a->q_rows, "q"}, {a->k, a->k_rows, "k"}, {a->v, a->k_rows, "v"}, {a->out, a->q_rows, "out"}, {g->d_out, a->q_rows, "d_out"}};
+    const Named grads[] = {q_named(a, g->d_q, "d_q"), k_named(a, g->d_k, "d_k"), k_named(a, g->d_v, "d_v")};
+    const Named in[] = {q_named(a, a->q, "q"), k_named(a, a->k, "k"), k_named(a, a->v, "v"), q_named(a, a->out, "out"), q_named(a, g->d_out, "d_out")};
     if (int rc = check_separate(ctx, what, grads, in)) return rc;
     const bl::PackedPlan plan = bl::plan_packed(*a, bl_compute_units_of(ctx));
     if (int rc = check_workspace(ctx, a, plan.backward_bytes, what)) return rc;

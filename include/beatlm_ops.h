@@ -60,7 +60,7 @@ int bl_ctx_create_on(int device_ordinal, void *stream, bl_ctx **out);
  * x, y, dy, dx, gamma and beta have the type `dtype`; the statistics and the
  * weights' gradients are f32, and so is every sum. Rows may be strided; the
  * width is 1 to BL_LAYER_NORM_MAX_COLS. y may be x, and dx may be dy or x
- * (with the same stride).
+ * (with the same stride); other overlaps of them are refused.
  * rows = 0 writes nothing but zeros to d_gamma and d_beta. The sums over rows
  * are made in a fixed order: equal calls give equal bits.
  * ------------------------------------------------------------------------ */
@@ -142,7 +142,7 @@ typedef struct {
     uint32_t head_dim;          /* 2 * pairs to 256 */
     uint32_t inverse;           /* 0 or 1 */
     const int32_t *positions;   /* [rows][axes] on the device; any int32 */
-    bl_heads q_in, q_out, k_in, k_out; /* out may be in itself (the same strides); otherwise they do not overlap */
+    bl_heads q_in, q_out, k_in, k_out; /* out may be in itself (the same strides); other overlaps of an output are refused */
 } bl_rotary_args;
 
 int bl_rotary(bl_ctx *ctx, const bl_rotary_table *table, const bl_rotary_args *args);
@@ -172,7 +172,9 @@ int bl_rotary(bl_ctx *ctx, const bl_rotary_table *table, const bl_rotary_args *a
  * may be anything too. Sums, statistics and scores are f32; for the matrix
  * cores the probabilities, and the scores' gradients, are rounded to the
  * tensors' type (f32 stays f32; f16 holds them times powers of two that keep
- * them in its range). What a call writes overlaps nothing else.
+ * them in its range). What a call writes overlaps nothing else that it
+ * touches: tensors that do are refused; lse, d_slopes and the workspace are not
+ * looked at.
  *
  * The offsets are device arrays, read when the kernels run (a captured graph
  * may be replayed with others); they are clamped to the tensors' rows, so
