@@ -142,3 +142,17 @@ def test_layer_norm_s_gradients_of_flat_rows_of_large_values(gpu, dtype, cols):
     assert_within(dx, want, half_step(torch_dtype) * want.abs() + off, "dx")
     assert torch.all(d_gamma == 0.0)
     assert_within(d_beta, dy.double().sum(0), F32 * (rows + 8) * dy.double().abs().sum(0), "d_beta")
+
+
+@pytest.mark.parametrize("axes", [0, 1, 2, 3])
+def test_few_tokens_over_many_blocks_of_keys(gpu, axes):
+    """f32, so many documents that no split cuts the keys short: a wave goes
+    through dozens of blocks with the next one's loads under way."""
+    t = Packed([(1 + i % 3, 1500 + 37 * i) for i in range(34)], "f32", 8, 8, 64, mask="causal", bias=0.02, axes=axes, gap=1)
+    a = t.args(gpu, False)
+    ops.attention(gpu, a)
+    t.check(["out", "lse"], False)
+    first = t.out.clone(), t.lse.clone()
+    for _ in range(5):
+        ops.attention(gpu, a)
+        assert torch.equal(t.out, first[0]) and torch.equal(t.lse, first[1])
