@@ -3,9 +3,10 @@
 // A thread owns VEC pairs of one row (or VEC channels of the copied tail) and
 // walks heads with them: it makes its VEC sines and cosines once, from the
 // table's 64-bit revolutions per position (pos * turns, its fraction taken in
-// 64 bits, so a position of 2^31 keeps an angle good to 2^-20 of f32's own
-// step), and every head of q and k then costs two 16-byte loads, six products
-// a pair and two stores. The bound is HBM: each channel in once, out once.
+// 64 bits: within |pos| 2^-54 revolutions, which is 2^-8 of f32's step at
+// positions of 2 million and four steps at 2^31; then one rounding to f32 and a
+// sine good to a few steps of 1), and every head of q and k then costs two
+// 16-byte loads, six products a pair and two stores. The bound is HBM: each channel in once, out once.
 // 32768 rows of 16 + 4 heads of 128, bf16: 74 us, 4.5 TB/s.
 #include "ops_device.hpp"
 

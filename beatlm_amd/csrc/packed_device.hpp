@@ -116,7 +116,10 @@ template <> struct Mma<float> {
 
 // KS values of a tile's registers (16-bit: registers 8 t .. 8 t + 7, f32:
 // 4 t .. 4 t + 3) as an operand of step t: the one rounding of probabilities
-// and scores' gradients to the tensors' type, which the matrix cores ask for.
+// and scores' gradients to the tensors' type, which the matrix cores ask for. It
+// averages out over keys: 2.1e-3 of the output's 2-norm where the output's own
+// rounding is 1.6e-3 (bf16, one token over 16326 keys), 3.0e-4 of d_q's where that is
+// 2.1e-4 (f16, 700 tokens). f32 is not rounded.
 template <typename T>
 __device__ __forceinline__ typename Mma<T>::Frag operand_of(const f32x16 &v, int t) {
     typename Mma<T>::Frag f;
@@ -286,9 +289,10 @@ __device__ __forceinline__ void store_partial(float *at, int half, const f32x16 
 
 // ---- scores ----
 //
-// In base two: x = log2(e) s, so probabilities are exp2(x - .). With a cap,
-// s = cap tanh(u), u = scale qk / cap. `factor` is what x is of a product, or
-// of its tanh.
+// In base two: x = log2(e) s, so probabilities are exp2(x - .), by the hardware's
+// exponential in every type: off by a step of f32, as its argument's own rounding
+// is from |x| = 1 on. With a cap, s = cap tanh(u), u = scale qk / cap. `factor` is
+// what x is of a product, or of its tanh.
 
 template <typename T, bool CAP> struct Scores {
     float factor;  // log2(e) scale, or log2(e) cap

@@ -22,7 +22,10 @@ PackedPlan plan_packed(const bl_packed_attention_args &a, uint32_t compute_units
     // keeping 64 streamed rows or more. The forward splits where the chip is
     // not covered once, then to four workgroups a compute unit (16 tokens over
     // 3449 to 16326 keys 71 us, two 83; packed images that cover it, 360 workgroups: 49
-    // us unsplit, 63 in three). The backward's causal rows are longer and its
+    // us unsplit, 63 in three). Decoding steps crosses the same line, though its
+    // sums are few: of ragged caches of 1724 to 8163 keys, 32 heads of 128 over 8,
+    // bf16, 31 (248 workgroups, in four) take 131 us, 32 (256, unsplit) 181; of
+    // caches of 8192 each, 193 and 197. The backward's causal rows are longer and its
     // workgroups larger: it splits to two a unit (8192 tokens, 260 workgroups:
     // d_k and d_v 0.81 ms in two, 1.3 unsplit; six texts, 468 workgroups, forward
     // and backward 112 us unsplit, 135 with the three a unit that split them).

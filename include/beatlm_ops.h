@@ -106,7 +106,8 @@ typedef struct {
  *   (a cos phi - b sin phi, a sin phi + b cos phi)
  * and channels beyond the pairs are copied. The gradient of a rotation is the
  * rotation by -phi: `inverse` 1 on the gradients. Angles are reduced in 64
- * bits, so far positions lose nothing; sines and products are f32.
+ * bits, to within |position| 2^-54 revolutions (less than f32's own step up to
+ * positions of 2^28); sines and products are f32.
  * ------------------------------------------------------------------------ */
 #define BL_ROTARY_MAX_PAIRS 128u
 enum {
