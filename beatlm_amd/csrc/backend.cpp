@@ -675,6 +675,11 @@ struct bl_kernels {
     // shares (their lifetimes are disjoint), and per kernel the entries its
     // split-k partial sums overwrite: writing one makes the others stale.
     std::vector<std::vector<uint32_t>> fold_alias, kernel_clobbers;
+    // On a host's stream that the host captures: the same for what its capture
+    // has taken so far, and which capture that is (0: none yet).
+    KvState captured_kv;
+    FoldState captured_folds;
+    unsigned long long capture = 0;
     std::vector<RangeGraph> graphs;
     // Graphs replay fixed launches: not used when a kernel of the program
     // rewrites a packed weight's source (the pack must rerun in between),
@@ -689,6 +694,8 @@ static void kernels_written(bl_kernels *k, uint32_t arena, uint64_t offset, uint
     k->kv = KvState{};
     // So may any folded LayerNorm's input.
     std::fill(k->fold_state.valid.begin(), k->fold_state.valid.end(), 0);
+    k->captured_kv = KvState{};
+    std::fill(k->captured_folds.valid.begin(), k->captured_folds.valid.end(), 0);
 }
 
 namespace {
@@ -1237,6 +1244,7 @@ void plan_folds(bl_kernels *ks, const bl_spec *specs, uint32_t n, const bl_bindi
     }
     ks->fold_state.valid.assign(ks->folds.size() * n_sets, 0);
     ks->fold_state.touched.assign(ks->folds.size() * n_sets, 0);
+    ks->captured_folds = ks->fold_state;
 }
 
 // The wave-split kernel's tile for a product, or -1 for the ring kernel: the
@@ -2330,15 +2338,48 @@ extern "C" const char *bl_kernels_label(const bl_kernels *k, uint32_t i) {
     return (k && i < k->kernels.size()) ? k->kernels[i].label.c_str() : nullptr;
 }
 
-// Packs a GEMM's B when its source may have changed since the last pack.
-static hipError_t refresh_pack(bl_kernels *k, const Launch &L, hipStream_t s) {
+// What the launches of a call follow and leave behind.
+struct Course {
+    KvState &kv;
+    FoldState &folds;
+    bool capturing;  // into a graph of the host's: nothing runs now, and it may be replayed at any time
+};
+
+// On a host's stream that is being captured, a capture's launches know only
+// of those before them in it, and what has run so far stays known as it is.
+// From the first capture on, a replay may have come before any call, so none
+// takes anything for held from the calls before it.
+static Course course_of(bl_kernels *k) {
+    const bl_ctx *ctx = k->ctx;
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (!ctx->owns_stream && ctx->stream && hipStreamGetCaptureInfo(ctx->stream, &status, &id) != hipSuccess) {
+        (void)hipGetLastError();
+        status = hipStreamCaptureStatusNone;
+    }
+    const auto forget = [](KvState &kv, FoldState &fs) {
+        kv = KvState{};
+        std::fill(fs.valid.begin(), fs.valid.end(), 0);
+    };
+    if (status != hipStreamCaptureStatusNone) {
+        if (k->capture != id) forget(k->captured_kv, k->captured_folds);
+        k->capture = id;
+        return {k->captured_kv, k->captured_folds, true};
+    }
+    if (k->capture) forget(k->kv, k->fold_state);
+    return {k->kv, k->fold_state, false};
+}
+
+// Packs a GEMM's B when its source may have changed since the last pack; into
+// a captured graph in any case, as it may change before a replay.
+static hipError_t refresh_pack(bl_kernels *k, const Launch &L, hipStream_t s, bool capturing = false) {
     Pack &pk = k->packs[L.pack];
-    if (!pk.dynamic && !pk.stale) return hipSuccess;
+    if (!capturing && !pk.dynamic && !pk.stale) return hipSuccess;
     PackArgs pa{pk.src, (char *)k->pack_buffer + pk.dst_offset, pk.k, pk.n, pk.k_pad, pk.n_pad,
                 pk.gamma.ptr, pk.beta.ptr, pk.bias.ptr,
                 pk.folded() ? (float *)((char *)k->pack_buffer + pk.vec_offset) : nullptr, pk.frag ? 1u : 0u, pk.tap_cols};
     hipError_t e = launch_pack(pa, pk.math, s);
-    if (e == hipSuccess) {
+    if (e == hipSuccess && !capturing) {
         pk.stale = false;
         k->packs_made++;
     }
@@ -2479,14 +2520,16 @@ extern "C" int bl_kernels_encode(bl_kernels *k, uint32_t kernel, uint32_t set, b
     if (kernel >= k->kernels.size()) return fail(k->ctx, BL_ERR_NO_SUCH_KERNEL, "there is no kernel %u", kernel);
     if (set >= k->sets) return fail(k->ctx, BL_ERR_NO_SUCH_SET, "there is no binding set %u", set);
     hipStream_t s = k->ctx->stream;
+    const Course course = course_of(k);
     int slice = -1;
+    if (timer && course.capturing) return fail(k->ctx, BL_ERR_INVALID_ARGUMENT, "a slice is not timed while the host captures its stream");
     if (timer) {
         int r = bl_timer_slice_begin(timer, tag, s, &slice);
         if (r) return r;
     }
     const Launch &L = k->kernels[kernel].per_set[set];
-    hipError_t e = L.pack >= 0 ? refresh_pack(k, L, s) : hipSuccess;
-    if (e == hipSuccess) e = run_one(k, kernel, set, s, k->kv, k->fold_state);
+    hipError_t e = L.pack >= 0 ? refresh_pack(k, L, s, course.capturing) : hipSuccess;
+    if (e == hipSuccess) e = run_one(k, kernel, set, s, course.kv, course.folds);
     if (e != hipSuccess) return hip_fail(k->ctx, e, k->kernels[kernel].label.c_str());
     if (timer && slice >= 0) bl_timer_slice_end(timer, slice, s);
     return BL_OK;
@@ -2585,10 +2628,11 @@ extern "C" int bl_kernels_encode_range(bl_kernels *k, uint32_t first, uint32_t c
             return BL_OK;
         }
     }
+    const Course course = course_of(k);
     for (uint32_t i = first; i < first + count; i++) {
         const Launch &L = k->kernels[i].per_set[set];
-        hipError_t e = L.pack >= 0 ? refresh_pack(k, L, s) : hipSuccess;
-        if (e == hipSuccess) e = run_one(k, i, set, s, k->kv, k->fold_state);
+        hipError_t e = L.pack >= 0 ? refresh_pack(k, L, s, course.capturing) : hipSuccess;
+        if (e == hipSuccess) e = run_one(k, i, set, s, course.kv, course.folds);
         if (e != hipSuccess) return hip_fail(k->ctx, e, k->kernels[i].label.c_str());
     }
     return BL_OK;
@@ -2609,6 +2653,8 @@ extern "C" int bl_kernels_time(bl_kernels *k, uint32_t kernel, uint32_t set, uin
     if (!k || !micros || repeats == 0) return BL_ERR_INVALID_ARGUMENT;
     if (kernel >= k->kernels.size()) return fail(k->ctx, BL_ERR_NO_SUCH_KERNEL, "there is no kernel %u", kernel);
     if (set >= k->sets) return fail(k->ctx, BL_ERR_NO_SUCH_SET, "there is no binding set %u", set);
+    const Course course = course_of(k);
+    if (course.capturing) return fail(k->ctx, BL_ERR_INVALID_ARGUMENT, "kernels are not timed while the host captures its stream");
     hipStream_t s = k->ctx->stream;
     hipEvent_t ev[2] = {nullptr, nullptr};
     hipError_t e = hipEventCreate(&ev[0]);
@@ -2618,7 +2664,7 @@ extern "C" int bl_kernels_time(bl_kernels *k, uint32_t kernel, uint32_t set, uin
     // kernel's scratch operands); the timed ones then run the kernel alone,
     // back to back, as it runs in its program.
     if (e == hipSuccess && L.pack >= 0) e = refresh_pack(k, L, s);
-    if (e == hipSuccess) e = run_one(k, kernel, set, s, k->kv, k->fold_state);
+    if (e == hipSuccess) e = run_one(k, kernel, set, s, course.kv, course.folds);
     if (e == hipSuccess) e = hipEventRecord(ev[0], s);
     for (uint32_t r = 0; r < repeats && e == hipSuccess; r++) e = launch(L, s);
     if (e == hipSuccess) e = hipEventRecord(ev[1], s);

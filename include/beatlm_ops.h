@@ -39,10 +39,14 @@ enum { BL_BF16 = 2 };
 
 /* bl_ctx_create over the host's stream (hipStream_t; NULL: the device's
  * default stream): everything the context launches goes there. The host keeps
- * the stream alive as long as the context and orders its own work on it as it
- * likes; destroying the context leaves the stream alone.
- * bl_kernels_encode_range on such a context launches one by one (the host may
- * be capturing the stream itself). A stream of another device is
+ * the stream alive as long as the context and what was made from it (arenas,
+ * kernels, timers) and orders its own work on it as it likes; destroying the
+ * context leaves the stream alone.
+ * bl_kernels_encode_range on such a context launches one by one, and the host
+ * may capture them into a graph of its own: a replay packs the program's
+ * weights again and takes nothing else for held from outside the graph, and
+ * after a capture no call takes anything for held from the calls before it.
+ * Nothing is timed in a capture. A stream of another device is
  * BL_ERR_INVALID_ARGUMENT. */
 int bl_ctx_create_on(int device_ordinal, void *stream, bl_ctx **out);
 
