@@ -17,6 +17,7 @@
 #include <string>
 #include <vector>
 
+#include "ctx.hpp"
 #include "spec.hpp"
 #include "timer.hpp"
 
@@ -79,6 +80,14 @@ bool profiler_attached() {
 }
 
 }  // namespace
+
+// The context's device, current: on a host's stream for the call alone.
+struct Bound {
+    DeviceScope scope;
+    explicit Bound(const bl_ctx *ctx) : scope(bl_hosts_device(ctx)) {
+        if (ctx->owns_stream) hipSetDevice(ctx->device);
+    }
+};
 
 struct bl_arenas {
     bl_ctx *ctx = nullptr;
@@ -213,6 +222,7 @@ extern "C" int bl_ctx_set_f32_math(bl_ctx *ctx, uint32_t mode) {
 
 extern "C" int bl_ctx_synchronize(bl_ctx *ctx) {
     if (!ctx) return BL_ERR_INVALID_ARGUMENT;
+    const DeviceScope scope(bl_hosts_device(ctx));
     hipError_t e = hipStreamSynchronize(ctx->stream);
     return e == hipSuccess ? BL_OK : hip_fail(ctx, e, "hipStreamSynchronize");
 }
@@ -245,6 +255,7 @@ bool bl_events_counted(bl_ctx *ctx, uint64_t n) {
 
 hipStream_t bl_stream_of(bl_ctx *ctx) { return ctx->stream; }
 int bl_device_of(const bl_ctx *ctx) { return ctx->device; }
+int bl_hosts_device(const bl_ctx *ctx) { return ctx->owns_stream ? -1 : ctx->device; }
 uint32_t bl_compute_units_of(const bl_ctx *ctx) { return ctx->compute_units; }
 uint32_t bl_f32_math_of(const bl_ctx *ctx) { return ctx->f32_math; }
 int bl_fail(bl_ctx *ctx, int code, const char *msg) { return fail(ctx, code, "%s", msg); }
@@ -254,7 +265,7 @@ int bl_fail(bl_ctx *ctx, int code, const char *msg) { return fail(ctx, code, "%s
 extern "C" int bl_arenas_create(bl_ctx *ctx, const uint64_t *sizes, uint32_t n, bl_arenas **out) {
     if (!ctx || !out || (n && !sizes)) return BL_ERR_INVALID_ARGUMENT;
     *out = nullptr;
-    hipSetDevice(ctx->device);
+    const Bound bound(ctx);
     bl_arenas *a = new bl_arenas();
     a->ctx = ctx;
     uint64_t total = 0;
@@ -286,7 +297,7 @@ extern "C" int bl_arenas_create(bl_ctx *ctx, const uint64_t *sizes, uint32_t n, 
 
 static void arenas_free(bl_arenas *a) {
     if (a->base) {
-        hipSetDevice(a->ctx->device);
+        const Bound bound(a->ctx);
         hipStreamSynchronize(a->ctx->stream);
         bl_device_free(a->ctx, a->base, a->total);
     }
@@ -319,7 +330,7 @@ extern "C" int bl_arenas_write(bl_arenas *a, uint32_t arena, uint64_t offset, co
     if (!a || (bytes && !src)) return BL_ERR_INVALID_ARGUMENT;
     if (int r = check_range(a, arena, offset, bytes)) return r;
     if (!bytes) return BL_OK;
-    hipSetDevice(a->ctx->device);
+    const Bound bound(a->ctx);
     hipError_t e = hipMemcpyAsync(a->base + a->offset[arena] + offset, src, bytes, hipMemcpyHostToDevice,
                                   a->ctx->stream);
     if (e == hipSuccess) e = hipStreamSynchronize(a->ctx->stream);
@@ -338,7 +349,7 @@ extern "C" int bl_arenas_read(bl_arenas *a, uint32_t arena, uint64_t offset, voi
     if (!a || (bytes && !dst)) return BL_ERR_INVALID_ARGUMENT;
     if (int r = check_range(a, arena, offset, bytes)) return r;
     if (!bytes) return BL_OK;
-    hipSetDevice(a->ctx->device);
+    const Bound bound(a->ctx);
     hipError_t e = hipMemcpyAsync(dst, a->base + a->offset[arena] + offset, bytes, hipMemcpyDeviceToHost,
                                   a->ctx->stream);
     if (e == hipSuccess) e = hipStreamSynchronize(a->ctx->stream);
@@ -1463,7 +1474,7 @@ extern "C" int bl_kernels_create_internal(bl_ctx *ctx, bl_arenas *arenas, const 
     if (!ctx || !arenas || !out || (n && !specs) || (n_sets && !sets) || (n_internal && !internal))
         return BL_ERR_INVALID_ARGUMENT;
     *out = nullptr;
-    hipSetDevice(ctx->device);
+    const Bound bound(ctx);
     const bl_binding_set identity{nullptr, 0};
     if (n_sets == 0) {
         sets = &identity;
@@ -2288,7 +2299,7 @@ extern "C" int bl_kernels_create_internal(bl_ctx *ctx, bl_arenas *arenas, const 
 
 extern "C" void bl_kernels_destroy(bl_kernels *k) {
     if (!k) return;
-    hipSetDevice(k->ctx->device);
+    const Bound bound(k->ctx);
     hipStreamSynchronize(k->ctx->stream);
     for (RangeGraph &g : k->graphs) hipGraphExecDestroy(g.exec);
     bl_device_free(k->ctx, k->workspace, k->workspace_bytes);
@@ -2325,7 +2336,7 @@ extern "C" int bl_kernels_fold_read(bl_kernels *k, uint32_t fold, uint32_t set, 
         have = fold_vec_bytes(pk.n_pad);
     }
     if (bytes > have) return BL_ERR_INVALID_ARGUMENT;
-    hipSetDevice(k->ctx->device);
+    const Bound bound(k->ctx);
     hipError_t e = hipStreamSynchronize(k->ctx->stream);
     if (e == hipSuccess) e = hipMemcpy(dst, src, bytes, hipMemcpyDeviceToHost);
     return e == hipSuccess ? BL_OK : hip_fail(k->ctx, e, "fold read");
@@ -2519,6 +2530,7 @@ extern "C" int bl_kernels_encode(bl_kernels *k, uint32_t kernel, uint32_t set, b
     if (!k) return BL_ERR_INVALID_ARGUMENT;
     if (kernel >= k->kernels.size()) return fail(k->ctx, BL_ERR_NO_SUCH_KERNEL, "there is no kernel %u", kernel);
     if (set >= k->sets) return fail(k->ctx, BL_ERR_NO_SUCH_SET, "there is no binding set %u", set);
+    const DeviceScope scope(bl_hosts_device(k->ctx));
     hipStream_t s = k->ctx->stream;
     const Course course = course_of(k);
     int slice = -1;
@@ -2594,6 +2606,7 @@ extern "C" int bl_kernels_encode_range(bl_kernels *k, uint32_t first, uint32_t c
     if ((uint64_t)first + count > k->kernels.size())
         return fail(k->ctx, BL_ERR_NO_SUCH_KERNEL, "there is no kernel %u", first + count - 1);
     if (set >= k->sets) return fail(k->ctx, BL_ERR_NO_SUCH_SET, "there is no binding set %u", set);
+    const DeviceScope scope(bl_hosts_device(k->ctx));
     hipStream_t s = k->ctx->stream;
     if (k->graphs_ok && count > 1) {
         // Stale packs are remade first, outside the graph (the graph holds the
@@ -2653,6 +2666,7 @@ extern "C" int bl_kernels_time(bl_kernels *k, uint32_t kernel, uint32_t set, uin
     if (!k || !micros || repeats == 0) return BL_ERR_INVALID_ARGUMENT;
     if (kernel >= k->kernels.size()) return fail(k->ctx, BL_ERR_NO_SUCH_KERNEL, "there is no kernel %u", kernel);
     if (set >= k->sets) return fail(k->ctx, BL_ERR_NO_SUCH_SET, "there is no binding set %u", set);
+    const DeviceScope scope(bl_hosts_device(k->ctx));
     const Course course = course_of(k);
     if (course.capturing) return fail(k->ctx, BL_ERR_INVALID_ARGUMENT, "kernels are not timed while the host captures its stream");
     hipStream_t s = k->ctx->stream;
@@ -2681,6 +2695,7 @@ extern "C" int bl_kernels_time(bl_kernels *k, uint32_t kernel, uint32_t set, uin
 extern "C" int bl_spin(bl_ctx *ctx, uint32_t micros) {
     if (!ctx) return BL_ERR_INVALID_ARGUMENT;
     if (!ctx->wall_clock_khz) return fail(ctx, BL_ERR_HIP, "the device reports no wall clock rate");
+    const DeviceScope scope(bl_hosts_device(ctx));
     uint64_t ticks = (uint64_t)micros * ctx->wall_clock_khz / 1000;
     hipError_t e = launch_spin(ticks, ctx->compute_units * 4, ctx->stream);
     return e == hipSuccess ? BL_OK : hip_fail(ctx, e, "spin");

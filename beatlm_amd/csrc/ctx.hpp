@@ -18,11 +18,16 @@ uint32_t bl_f32_math_of(const bl_ctx *ctx);
 // Sets the context's message (no allocation for messages under 512 bytes).
 int bl_fail(bl_ctx *ctx, int code, const char *msg);
 
-// Makes `device` current for a call and restores the caller's device after.
+// The context's device where its stream is the host's, else -1.
+int bl_hosts_device(const bl_ctx *ctx);
+
+// Makes `device` current for a call and restores the caller's device after
+// (-1: leaves it alone).
 struct DeviceScope {
     int prev = -1;
     hipError_t status = hipSuccess;
     explicit DeviceScope(int device) {
+        if (device < 0) return;
         status = hipGetDevice(&prev);
         if (status == hipSuccess && prev != device) status = hipSetDevice(device);
         else if (status == hipSuccess) prev = -1;  // already current: nothing to restore

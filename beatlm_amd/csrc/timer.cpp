@@ -61,6 +61,7 @@ static constexpr uint32_t TIMER_MAX_SLICES = BLS_TIMER_MAX_SLICES;  // what time
 extern "C" int bl_timer_create(bl_ctx *ctx, uint32_t max_slices, bl_timer **out) {
     if (!ctx || !out) return BL_ERR_INVALID_ARGUMENT;
     *out = nullptr;
+    const DeviceScope scope(bl_hosts_device(ctx));
     if (max_slices == 0 || max_slices > TIMER_MAX_SLICES)
         return bl_fail(ctx, BL_ERR_INVALID_ARGUMENT, "slice capacity outside 1..=4096");
     auto *t = new bl_timer();
@@ -95,6 +96,7 @@ extern "C" int bl_timer_create(bl_ctx *ctx, uint32_t max_slices, bl_timer **out)
 
 extern "C" void bl_timer_destroy(bl_timer *t) {
     if (!t) return;
+    const DeviceScope scope(bl_hosts_device(t->ctx));
     hipStreamSynchronize(bl_stream_of(t->ctx));
     for (Slot &s : t->slots) {
         for (hipEvent_t e : s.events)
@@ -161,6 +163,7 @@ extern "C" int bl_timer_render_begin(bl_timer *t) {
     t->render_begun = true;
     if (t->open < 0) return BL_OK;  // untimed frame
     Slot &s = t->slots[t->open];
+    const DeviceScope scope(bl_hosts_device(t->ctx));
     if (hipEventRecord(s.render[0], bl_stream_of(t->ctx)) != hipSuccess)
         return bl_fail(t->ctx, BL_ERR_HIP, "hipEventRecord");
     s.render_state = 1;
@@ -173,6 +176,7 @@ extern "C" int bl_timer_render_end(bl_timer *t) {
     if (t->open < 0) return BL_OK;
     Slot &s = t->slots[t->open];
     if (s.render_state != 1) return bl_fail(t->ctx, BL_ERR_INVALID_ARGUMENT, "the render pass was not begun");
+    const DeviceScope scope(bl_hosts_device(t->ctx));
     if (hipEventRecord(s.render[1], bl_stream_of(t->ctx)) != hipSuccess)
         return bl_fail(t->ctx, BL_ERR_HIP, "hipEventRecord");
     s.render_state = 2;
@@ -187,6 +191,7 @@ extern "C" int bl_timer_resolve(bl_timer *t, uint64_t *resolved) {
     if (t->open < 0) return BL_OK;
     const uint32_t i = (uint32_t)t->open;
     t->open = -1;
+    const DeviceScope scope(bl_hosts_device(t->ctx));
     if (hipEventRecord(t->slots[i].done, bl_stream_of(t->ctx)) != hipSuccess) {
         t->ring.release(i);
         return bl_fail(t->ctx, BL_ERR_HIP, "hipEventRecord");

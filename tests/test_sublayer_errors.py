@@ -14,7 +14,9 @@ STAND_IN = r"""
 #include <hip/hip_runtime_api.h>
 #include <string.h>
 extern "C" {
-int launches = 0, failing = -1, current = 0, refused_streams = 0;
+int launches = 0, failing = -1, current = 0;
+int calls = 0, elsewhere = 0, at_device = 0;  // calls that ask for a current device, and those of them on another
+static hipError_t on_device(void) { calls++; elsewhere += current != at_device; return hipSuccess; }
 hipError_t pending = hipSuccess;  // the host thread's last error
 static hipError_t failed(hipError_t e) { return pending = e; }
 hipError_t hipGetLastError(void) { const hipError_t e = pending; pending = hipSuccess; return e; }
@@ -22,7 +24,16 @@ hipError_t hipPeekAtLastError(void) { return pending; }
 hipError_t hipGetDeviceCount(int *n) { *n = 2; return hipSuccess; }
 hipError_t hipGetDevice(int *d) { *d = current; return hipSuccess; }
 hipError_t hipSetDevice(int d) { if (d < 0 || d > 1) return failed(hipErrorInvalidDevice); current = d; return hipSuccess; }
-hipError_t hipGetDeviceProperties(hipDeviceProp_t *p, int) { memset(p, 0, sizeof *p); p->multiProcessorCount = 256; p->warpSize = 64; return hipSuccess; }
+hipError_t hipGetDeviceProperties(hipDeviceProp_t *p, int) {
+    memset(p, 0, sizeof *p);
+    p->multiProcessorCount = 256;
+    p->warpSize = 64;
+    p->totalGlobalMem = 1 << 26;
+    p->sharedMemPerBlock = 1 << 16;
+    p->maxThreadsPerBlock = 1024;
+    for (int n = 0; n < 3; n++) p->maxThreadsDim[n] = 1024, p->maxGridSize[n] = 1 << 30;
+    return hipSuccess;
+}
 hipError_t hipDeviceGetAttribute(int *v, hipDeviceAttribute_t, int) { *v = 100000; return hipSuccess; }
 // A stream's address is its device's number times 16, and 16; others are no streams.
 hipError_t hipStreamGetDevice(hipStream_t s, hipDevice_t *d) {
@@ -30,7 +41,23 @@ hipError_t hipStreamGetDevice(hipStream_t s, hipDevice_t *d) {
     *d = (int)((size_t)s / 16) - 1;
     return hipSuccess;
 }
+// What a program needs beside that: memory, copies and events.
+static char memory[1 << 26];
+hipError_t hipMalloc(void **p, size_t n) { *p = memory; return n > sizeof memory ? failed(hipErrorOutOfMemory) : on_device(); }
+hipError_t hipFree(void *) { return on_device(); }
+hipError_t hipMemcpyAsync(void *, const void *, size_t, hipMemcpyKind, hipStream_t) { return on_device(); }
+hipError_t hipMemsetAsync(void *, int, size_t, hipStream_t) { return on_device(); }
+hipError_t hipStreamSynchronize(hipStream_t) { return on_device(); }
+hipError_t hipEventCreate(hipEvent_t *e) { *e = (hipEvent_t)memory; return on_device(); }
+hipError_t hipEventDestroy(hipEvent_t) { return hipSuccess; }
+hipError_t hipEventRecord(hipEvent_t, hipStream_t) { return on_device(); }
+hipError_t hipEventSynchronize(hipEvent_t) { return hipSuccess; }
+hipError_t hipEventElapsedTime(float *ms, hipEvent_t, hipEvent_t) { *ms = 1.0f; return hipSuccess; }
+hipError_t hipStreamGetCaptureInfo(hipStream_t, hipStreamCaptureStatus *s, unsigned long long *) { *s = hipStreamCaptureStatusNone; return hipSuccess; }
+hipError_t __hipPushCallConfiguration(dim3, dim3, size_t, hipStream_t) { return hipSuccess; }
+hipError_t __hipPopCallConfiguration(dim3 *, dim3 *, size_t *, hipStream_t *) { return hipSuccess; }
 hipError_t hipLaunchKernel(const void *, dim3, dim3, void **, size_t, hipStream_t) {
+    on_device();
     return launches++ == failing ? failed(hipErrorOutOfMemory) : hipSuccess;
 }
 }
@@ -140,4 +167,50 @@ for stream in (32, 48):  # another device's, and none
     else:
         raise AssertionError(stream)
     assert (pending.value, current.value) == (0, 0), stream
+""")
+
+
+def test_programs_on_a_host_s_stream_leave_the_current_device(run):
+    """Everything that a context over another device's stream does happens on
+    that device, the default stream's work too, and leaves the host's current."""
+    run("""
+import numpy as np
+from beatlm_amd import ir
+calls, elsewhere, at_device = (C.c_int.in_dll(stand_in, n) for n in ("calls", "elsewhere", "at_device"))
+for mine, device, stream in ((0, 0, 16), (0, 1, 32), (1, 0, 0), (0, 1, 0)):
+    current.value, at_device.value = mine, device
+    launches.value = calls.value = elsewhere.value = 0
+    def same(what):
+        assert (current.value, elsewhere.value) == (mine, 0), (mine, device, stream, what, current.value, elsewhere.value)
+    c = hip.Context(device, stream=stream)
+    g = ir.Graph()
+    g.tensor(0, ir.INPUT, 33 * 64)
+    for t in (1, 2):
+        g.tensor(t, ir.WEIGHT, 64)
+    g.tensor(3, ir.OUTPUT, 33 * 64)
+    g.push(ir.op(ir.OP_LAYER_NORM, [0, 1, 2], [33, 64], 1e-6), 3)
+    prep = ir.prepare(c, g)
+    same("made")
+    prep.write(1, np.ones(64, np.float32))
+    same("written")
+    prep.run()
+    same("run")
+    t = hip.Timer(c, 4)
+    same("a timer")
+    t.begin_frame(1)
+    prep.kernels.encode(0, 0, t, 7)
+    t.render_begin()
+    t.render_end()
+    t.resolve()
+    same("encoded and timed")
+    prep.kernels.time(0, repeats=2)
+    same("timed alone")
+    c.synchronize()
+    prep.read(3)
+    same("read")
+    t.close()
+    prep.close()
+    c.close()
+    same("closed")
+    assert launches.value >= 5 and calls.value > launches.value, (launches.value, calls.value)
 """)
