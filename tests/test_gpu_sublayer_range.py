@@ -156,3 +156,24 @@ def test_few_tokens_over_many_blocks_of_keys(gpu, axes):
     for _ in range(5):
         ops.attention(gpu, a)
         assert torch.equal(t.out, first[0]) and torch.equal(t.lse, first[1])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("keys", [1, 300])
+def test_statistics_near_zero_keep_their_digits(gpu, dtype, keys):
+    """Scores and lse of 2^-12 and less: lse is the score itself over one key, and
+    keys whose number the bias of the first cancels leave nothing else."""
+    t = Packed([(1, keys)] * 20, dtype, 2, 1, 16, scale=1.0)
+    t.q.zero_()
+    t.k.zero_()
+    t.q[..., 0] = 2.0**-6
+    t.k[:, :, 0] = (torch.rand(t.k_rows, 1, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)) * 2.0**-6).to(t.torch_dtype)
+    if keys > 1:  # all but the first of a document far below it
+        t.q[..., 1] = 64.0
+        t.k[:, :, 1] = -8.0
+        t.k[0::keys, :, 1] = 0.0
+    ops.attention(gpu, t.args(gpu, False))
+    first = t.k[0::keys, 0].double()
+    want = (t.q[..., 0].double() * first[:, None, 0]).T  # one product, exact in f32
+    # into base two, and out of it again: a few roundings of it, and the hardware's log2 of a sum of 1
+    assert_within(t.lse, want, 6 * F32 * want.abs(), "lse")
