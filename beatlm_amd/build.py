@@ -48,8 +48,15 @@ SOURCES = [
     "k_packed_f32.hip",
     "k_packed_f16.hip",
     "k_packed_bf16.hip",
+    "k_heads.hip",
+    "k_cache.hip",
+    "k_paged_f32.hip",
+    "k_paged_f16.hip",
+    "k_paged_bf16.hip",
     "packed_plan.cpp",
+    "paged_plan.cpp",
     "ops.cpp",
+    "cache_ops.cpp",
     "backend.cpp",
     "timer.cpp",
     "ring.cpp",

@@ -1,6 +1,8 @@
 // The packed attention sublayer's operators (include/beatlm_ops.h): what the
 // host side (ops.cpp, packed_plan.cpp) hands to the kernels (k_norm.hip,
-// k_rotary.hip, k_packed.inc). The launch functions check nothing: ops.cpp has.
+// k_rotary.hip, k_packed.inc), and cache_ops.cpp and paged_plan.cpp to theirs
+// (k_heads.hip, k_cache.hip, k_paged.inc). The launch functions check nothing:
+// ops.cpp and cache_ops.cpp have.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -75,5 +77,56 @@ hipError_t launch_packed_backward(const PackedParams &p, const PackedPlan &plan,
 // One element type each (k_packed_*.hip).
 template <typename T> hipError_t packed_forward(const PackedParams &p, const PackedPlan &plan, hipStream_t s);
 template <typename T> hipError_t packed_backward(const PackedParams &p, const PackedPlan &plan, hipStream_t s);
+
+// ---- norms of each head with their rotary positions ----
+
+struct HeadsParams {
+    bl_rotary_table table;   // pairs 0: no rotation
+    const int32_t *positions;
+    const void *q_gamma, *k_gamma;  // null: ones
+    bl_heads q_in, q_out, k_in, k_out;
+    bl_heads dq_out, dk_out, dq_in, dk_in;
+    float *partial;          // [groups][2][head_dim]: the weights' gradients of one workgroup's rows
+    float *d_q_gamma, *d_k_gamma;
+    uint32_t rows, q_heads, k_heads, head_dim, norm;
+    float epsilon;
+    uint32_t groups;         // workgroups that walk the rows of the backward
+    uint32_t vec;            // elements of an access: 16 bytes, 8 or one element, as everything is aligned
+};
+constexpr uint32_t HEADS_BACKWARD_GROUPS = 4;  // a compute unit
+hipError_t launch_heads_forward(const HeadsParams &p, uint32_t dtype, uint32_t compute_units, hipStream_t s);
+hipError_t launch_heads_backward(const HeadsParams &p, uint32_t dtype, uint32_t compute_units, hipStream_t s);
+
+// ---- the cache of pages ----
+
+struct AppendParams {
+    HeadsParams h;           // k_out is not used
+    bl_heads v_in;
+    bl_paged_cache cache;
+    const int32_t *q_offsets;
+    uint32_t documents;
+};
+hipError_t launch_cache_append(const AppendParams &p, uint32_t dtype, uint32_t compute_units, hipStream_t s);
+hipError_t launch_cache_read(const bl_cache_read_args &a, uint32_t compute_units, hipStream_t s);
+
+// ---- attention over pages ----
+
+struct PagedPlan {
+    uint32_t blocks;    // of 16 (query, head of a group) places in a workgroup
+    uint32_t splits;    // workgroups that share a document's keys
+    uint32_t tile_dim;  // channels of the kernels' tiles: 64 or 128
+    uint64_t partial_bytes, stats_bytes;
+};
+struct PagedParams {
+    bl_paged_attention_args a;
+    uint32_t splits;
+    uint32_t page_magic;  // ceil(2^32 / page_rows): n / page_rows is the upper half of n times it, up to BL_CACHE_MAX_KEYS
+    float *partial;       // [splits][places][tile_dim]; places = q_rows * q_heads
+    float *stats;         // [splits][places][2]
+};
+PagedPlan plan_paged(const bl_paged_attention_args &a, uint32_t compute_units);
+hipError_t launch_paged(const bl_paged_attention_args &a, const PagedPlan &plan, hipStream_t s);
+// One element type each (k_paged_*.hip).
+template <typename T> hipError_t paged_attention(const PagedParams &p, const PagedPlan &plan, hipStream_t s);
 
 }  // namespace bl

@@ -1,6 +1,8 @@
 """ctypes binding of the packed attention sublayer's operators
-(include/beatlm_ops.h): LayerNorm, rotary positions of several axes and
-attention over packed documents, with their gradients.
+(include/beatlm_ops.h): LayerNorm, rotary positions of several axes, attention
+over packed documents and norms of each head with its rotary positions, with
+their gradients; and a cache of keys in pages, what appends to it, reads it back
+and attends over it.
 
 The argument structs hold device addresses (an arena's `device_ptr`, another
 library's buffer) and are read during the call alone, so a program keeps one
@@ -20,10 +22,16 @@ BF16 = 2  # beside hip.F32 and hip.F16, in these operators alone
 LAYER_NORM_MAX_COLS = 16384
 ROTARY_MAX_PAIRS = 128
 ATTENTION_MAX_HEAD_DIM = 128
+HEAD_NORM_MAX_HEAD_DIM = 256
+CACHE_MAX_PAGE_ROWS = 256
+CACHE_MAX_KEYS = 1 << 24
+CACHE_GROUP = 32
 
 ROTARY_HALVES, ROTARY_NEIGHBOURS = 0, 1
 ROTARY_SHARED, ROTARY_PER_AXIS = 0, 1
 MASK_NONE, MASK_CAUSAL, MASK_PREFIX = 0, 1, 2
+HEAD_NORM_NONE, HEAD_NORM_RMS, HEAD_NORM_CENTRED = 0, 1, 2
+CACHE_PLAIN, CACHE_INT4 = 0, 1
 
 _U32, _U64, _F32, _P = C.c_uint32, C.c_uint64, C.c_float, C.c_void_p
 
@@ -77,6 +85,55 @@ class AttentionGrads(C.Structure):
     _fields_ = [("d_out", Heads), ("d_q", Heads), ("d_k", Heads), ("d_v", Heads), ("d_slopes", _P)]
 
 
+class HeadNormArgs(C.Structure):
+    _fields_ = [
+        ("dtype", _U32), ("rows", _U32), ("q_heads", _U32), ("k_heads", _U32), ("head_dim", _U32), ("norm", _U32), ("epsilon", _F32),
+        ("positions", _P), ("q_gamma", _P), ("k_gamma", _P), ("q_in", Heads), ("q_out", Heads), ("k_in", Heads), ("k_out", Heads),
+    ]
+
+
+class HeadNormGrads(C.Structure):
+    _fields_ = [
+        ("dq_out", Heads), ("dk_out", Heads), ("dq_in", Heads), ("dk_in", Heads),
+        ("d_q_gamma", _P), ("d_k_gamma", _P), ("workspace", _P), ("workspace_bytes", _U64),
+    ]
+
+
+class Pages(C.Structure):
+    """Rows of (page, row, head) at a device address; strides in bytes."""
+
+    _fields_ = [("data", _P), ("page_stride", _U64), ("row_stride", _U64), ("head_stride", _U64)]
+
+
+class PagedCache(C.Structure):
+    _fields_ = [
+        ("kind", _U32), ("pages", _U32), ("page_rows", _U32), ("max_pages", _U32), ("table", _P), ("lengths", _P), ("k", Pages), ("v", Pages),
+    ]
+
+
+class CacheAppendArgs(C.Structure):
+    _fields_ = [
+        ("dtype", _U32), ("rows", _U32), ("documents", _U32), ("q_heads", _U32), ("kv_heads", _U32), ("head_dim", _U32), ("norm", _U32), ("epsilon", _F32),
+        ("q_offsets", _P), ("positions", _P), ("q_gamma", _P), ("k_gamma", _P),
+        ("q_in", Heads), ("q_out", Heads), ("k_in", Heads), ("v_in", Heads), ("cache", PagedCache),
+    ]
+
+
+class CacheReadArgs(C.Structure):
+    _fields_ = [
+        ("dtype", _U32), ("rows", _U32), ("documents", _U32), ("kv_heads", _U32), ("head_dim", _U32),
+        ("offsets", _P), ("first", _P), ("k_out", Heads), ("v_out", Heads), ("cache", PagedCache),
+    ]
+
+
+class PagedAttentionArgs(C.Structure):
+    _fields_ = [
+        ("dtype", _U32), ("q_heads", _U32), ("kv_heads", _U32), ("head_dim", _U32), ("q_rows", _U32), ("documents", _U32),
+        ("mask", _U32), ("window", _U32), ("max_keys", _U32), ("scale", _F32), ("softcap", _F32),
+        ("q_offsets", _P), ("q", Heads), ("out", Heads), ("lse", _P), ("cache", PagedCache), ("workspace", _P), ("workspace_bytes", _U64),
+    ]
+
+
 _SIG = {
     "bl_layer_norm": (C.c_int, [_P, C.POINTER(LayerNormArgs)]),
     "bl_layer_norm_backward_workspace": (C.c_int, [_P, C.POINTER(LayerNormArgs), C.POINTER(_U64)]),
@@ -86,6 +143,13 @@ _SIG = {
     "bl_packed_attention_workspace": (C.c_int, [_P, C.POINTER(AttentionArgs), _U32, C.POINTER(_U64)]),
     "bl_packed_attention": (C.c_int, [_P, C.POINTER(AttentionArgs)]),
     "bl_packed_attention_backward": (C.c_int, [_P, C.POINTER(AttentionArgs), C.POINTER(AttentionGrads)]),
+    "bl_head_norm_rotary": (C.c_int, [_P, C.POINTER(RotaryTable), C.POINTER(HeadNormArgs)]),
+    "bl_head_norm_rotary_backward_workspace": (C.c_int, [_P, C.POINTER(HeadNormArgs), C.POINTER(_U64)]),
+    "bl_head_norm_rotary_backward": (C.c_int, [_P, C.POINTER(RotaryTable), C.POINTER(HeadNormArgs), C.POINTER(HeadNormGrads)]),
+    "bl_cache_append": (C.c_int, [_P, C.POINTER(RotaryTable), C.POINTER(CacheAppendArgs)]),
+    "bl_cache_read": (C.c_int, [_P, C.POINTER(CacheReadArgs)]),
+    "bl_paged_attention_workspace": (C.c_int, [_P, C.POINTER(PagedAttentionArgs), C.POINTER(_U64)]),
+    "bl_paged_attention": (C.c_int, [_P, C.POINTER(PagedAttentionArgs)]),
 }
 _bound = None
 
@@ -149,3 +213,43 @@ def attention(ctx: Context, args: AttentionArgs) -> None:
 
 def attention_backward(ctx: Context, args: AttentionArgs, grads: AttentionGrads) -> None:
     ctx.check(_lib().bl_packed_attention_backward(ctx.handle, C.byref(args), C.byref(grads)))
+
+
+def _table(table: RotaryTable | None):
+    return None if table is None else C.byref(table)
+
+
+def head_norm_rotary(ctx: Context, table: RotaryTable | None, args: HeadNormArgs) -> None:
+    """table None: norms alone."""
+    ctx.check(_lib().bl_head_norm_rotary(ctx.handle, _table(table), C.byref(args)))
+
+
+def head_norm_rotary_backward_workspace(ctx: Context, args: HeadNormArgs) -> int:
+    """Bytes of the workspace head_norm_rotary_backward needs for these sizes."""
+    n = _U64()
+    ctx.check(_lib().bl_head_norm_rotary_backward_workspace(ctx.handle, C.byref(args), C.byref(n)))
+    return int(n.value)
+
+
+def head_norm_rotary_backward(ctx: Context, table: RotaryTable | None, args: HeadNormArgs, grads: HeadNormGrads) -> None:
+    ctx.check(_lib().bl_head_norm_rotary_backward(ctx.handle, _table(table), C.byref(args), C.byref(grads)))
+
+
+def cache_append(ctx: Context, table: RotaryTable | None, args: CacheAppendArgs) -> None:
+    """table None: no rotation."""
+    ctx.check(_lib().bl_cache_append(ctx.handle, _table(table), C.byref(args)))
+
+
+def cache_read(ctx: Context, args: CacheReadArgs) -> None:
+    ctx.check(_lib().bl_cache_read(ctx.handle, C.byref(args)))
+
+
+def paged_attention_workspace(ctx: Context, args: PagedAttentionArgs) -> int:
+    """Bytes of the workspace paged_attention needs for these sizes."""
+    n = _U64()
+    ctx.check(_lib().bl_paged_attention_workspace(ctx.handle, C.byref(args), C.byref(n)))
+    return int(n.value)
+
+
+def paged_attention(ctx: Context, args: PagedAttentionArgs) -> None:
+    ctx.check(_lib().bl_paged_attention(ctx.handle, C.byref(args)))
