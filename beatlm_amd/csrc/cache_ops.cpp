@@ -1,5 +1,5 @@
 // The host side of the norms of heads and of the cache of pages
-// (include/beatlm_ops.h): every check of a call's arguments, and the launch on
+// (include/beatlm_cache.h): every check of a call's arguments, and the launch on
 // the context's stream. Nothing here allocates or waits.
 #include "ops.hpp"
 #include "ops_checks.hpp"

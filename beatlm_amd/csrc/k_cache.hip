@@ -1,6 +1,6 @@
 // New keys and values into a cache of pages, with the keys' norm and rotary
 // positions on the way and the queries' beside them, and the way back to packed
-// rows (include/beatlm_ops.h).
+// rows (include/beatlm_cache.h).
 //
 // First a few threads a row find its document, its place and its page, then the
 // workgroup makes the rows' sines once, then every head is a few threads' as in
@@ -77,6 +77,11 @@ __device__ __forceinline__ float quad_min(float v) {
     return fminf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x4E, 0xF, 0xF, false)));
 }
 __device__ __forceinline__ uint32_t half_bits(float v) { return __builtin_bit_cast(uint16_t, (_Float16)v); }
+// To f32: a rounding that the compiler would otherwise join with one to f16 behind it.
+__device__ __forceinline__ float rounded_once(double v) {
+#pragma clang fp contract(off)
+    return (float)v;
+}
 
 // 8 channels of a group that the lane's quad shares, to their codes, and from
 // the quad's first lane the group's step and low. Both round once from f32, and
@@ -93,7 +98,7 @@ __device__ __forceinline__ void store_codes(const float (&x)[8], char *row, uint
     least = quad_min(least);
     most = -quad_min(-most);
     bad = -quad_min(-bad);
-    const uint32_t low_bits = half_bits(least), step_bits = bad != 0.0f ? 0x7e00u : half_bits((float)(((double)most - (double)least) / 15.0));
+    const uint32_t low_bits = half_bits(least), step_bits = bad != 0.0f ? 0x7e00u : half_bits(rounded_once(((double)most - (double)least) / 15.0));
     const double low = (float)__builtin_bit_cast(_Float16, (uint16_t)low_bits), step = (float)__builtin_bit_cast(_Float16, (uint16_t)step_bits);
     uint32_t codes = 0;
 #pragma unroll

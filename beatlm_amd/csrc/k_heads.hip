@@ -1,5 +1,5 @@
 // Norms of each head of queries and keys with their rotary positions, and the
-// gradients (include/beatlm_ops.h).
+// gradients (include/beatlm_cache.h).
 //
 // A head's channels are in registers from the load to the store (heads_device.hpp):
 // its sums are over the few lanes that have it. The bound is HBM: forward each

@@ -1,4 +1,4 @@
-// The packed attention sublayer's operators (include/beatlm_ops.h): what the
+// The packed attention sublayer's operators (include/beatlm_ops.h, include/beatlm_cache.h): what the
 // host side (ops.cpp, packed_plan.cpp) hands to the kernels (k_norm.hip,
 // k_rotary.hip, k_packed.inc), and cache_ops.cpp and paged_plan.cpp to theirs
 // (k_heads.hip, k_cache.hip, k_paged.inc). The launch functions check nothing:
@@ -7,7 +7,7 @@
 
 #include <hip/hip_runtime.h>
 
-#include "../../include/beatlm_ops.h"
+#include "../../include/beatlm_cache.h"
 
 namespace bl {
 

@@ -1,4 +1,4 @@
-// The plan of attention over pages (include/beatlm_ops.h): how many places a
+// The plan of attention over pages (include/beatlm_cache.h): how many places a
 // workgroup has, into how many splits the keys are cut and what the workspace
 // holds, from the sizes alone, so a workspace made for them fits every call.
 #include "ops.hpp"

@@ -1,8 +1,8 @@
 """ctypes binding of the packed attention sublayer's operators
-(include/beatlm_ops.h): LayerNorm, rotary positions of several axes, attention
-over packed documents and norms of each head with its rotary positions, with
-their gradients; and a cache of keys in pages, what appends to it, reads it back
-and attends over it.
+(include/beatlm_ops.h): LayerNorm, rotary positions of several axes and
+attention over packed documents, with their gradients; and of those beside them
+(include/beatlm_cache.h): norms of each head with its rotary positions, and a
+cache of keys in pages, what appends to it, reads it back and attends over it.
 
 The argument structs hold device addresses (an arena's `device_ptr`, another
 library's buffer) and are read during the call alone, so a program keeps one
@@ -143,6 +143,9 @@ _SIG = {
     "bl_packed_attention_workspace": (C.c_int, [_P, C.POINTER(AttentionArgs), _U32, C.POINTER(_U64)]),
     "bl_packed_attention": (C.c_int, [_P, C.POINTER(AttentionArgs)]),
     "bl_packed_attention_backward": (C.c_int, [_P, C.POINTER(AttentionArgs), C.POINTER(AttentionGrads)]),
+}
+# include/beatlm_cache.h
+_CACHE_SIG = {
     "bl_head_norm_rotary": (C.c_int, [_P, C.POINTER(RotaryTable), C.POINTER(HeadNormArgs)]),
     "bl_head_norm_rotary_backward_workspace": (C.c_int, [_P, C.POINTER(HeadNormArgs), C.POINTER(_U64)]),
     "bl_head_norm_rotary_backward": (C.c_int, [_P, C.POINTER(RotaryTable), C.POINTER(HeadNormArgs), C.POINTER(HeadNormGrads)]),
@@ -158,7 +161,7 @@ def _lib():
     global _bound
     if _bound is None:
         h = lib()
-        for name, (res, args) in _SIG.items():
+        for name, (res, args) in {**_SIG, **_CACHE_SIG}.items():
             fn = getattr(h, name)
             fn.restype = res
             fn.argtypes = args
