@@ -111,18 +111,20 @@ hipError_t launch_cache_read(const bl_cache_read_args &a, uint32_t compute_units
 
 // ---- attention over pages ----
 
+constexpr uint32_t PAGED_CHUNK_BLOCKS = 8;
 struct PagedPlan {
-    uint32_t blocks;    // of 16 (query, head of a group) places in a workgroup
-    uint32_t splits;    // workgroups that share a document's keys
+    uint32_t blocks;    // of 16 (query, head of a group) places in a workgroup: 1, 2 or PAGED_CHUNK_BLOCKS
+    uint32_t share;     // of chunks: keys of a workgroup, from the first that its places see
+    uint32_t splits;    // workgroups that share a document's keys; of chunks the longest one's, and the last takes what is left of a longer one
     uint32_t tile_dim;  // channels of the kernels' tiles: 64 or 128
     uint64_t partial_bytes, stats_bytes;
 };
 struct PagedParams {
     bl_paged_attention_args a;
-    uint32_t splits;
+    uint32_t share, splits;
     uint32_t page_magic;  // ceil(2^32 / page_rows): n / page_rows is the upper half of n times it, up to BL_CACHE_MAX_KEYS
     float *partial;       // [splits][places][tile_dim]; places = q_rows * q_heads
-    float *stats;         // [splits][places][2]
+    float *stats;         // [splits][places][4]: maximum, sum, and how many splits the place has
 };
 PagedPlan plan_paged(const bl_paged_attention_args &a, uint32_t compute_units);
 hipError_t launch_paged(const bl_paged_attention_args &a, const PagedPlan &plan, hipStream_t s);

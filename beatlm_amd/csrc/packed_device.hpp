@@ -297,6 +297,7 @@ __device__ __forceinline__ void store_partial(float *at, int half, const f32x16 
 template <typename T, bool CAP> struct Scores {
     float factor;  // log2(e) scale, or log2(e) cap
     float inner;   // scale / cap
+    Scores() = default;
     // `ordered`: for q whose sign the caller has changed where scale is
     // negative, so that x grows with the product (and a scale of zero keeps a
     // hidden -inf what it is).

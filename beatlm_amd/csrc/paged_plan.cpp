@@ -14,18 +14,35 @@ PagedPlan plan_paged(const bl_paged_attention_args &a, uint32_t compute_units) {
     plan.tile_dim = a.head_dim <= 64 ? 64 : 128;
     const uint64_t group = a.q_heads / a.kv_heads, places = (uint64_t)a.q_rows * a.q_heads;
     const uint64_t average = ((uint64_t)a.q_rows * group + a.documents - 1) / a.documents;
-    plan.blocks = average <= 16 ? 1 : average <= 32 ? 2 : 4;
+    plan.blocks = average <= 16 ? 1 : average <= 32 ? 2 : PAGED_CHUNK_BLOCKS;
     const uint64_t table = (uint64_t)a.cache.max_pages * a.cache.page_rows;
     uint64_t keys = a.max_keys && a.max_keys < table ? a.max_keys : table;
     if (a.window && (uint64_t)a.window + a.q_rows < keys) keys = (uint64_t)a.window + a.q_rows;
     // Workgroups without splits, and a last, partial one a document.
-    const uint64_t whole = ((uint64_t)a.q_rows * group / (16 * plan.blocks) + a.documents) * a.kv_heads;
-    const uint64_t wanted = whole < 4ull * compute_units ? (4ull * compute_units + whole - 1) / whole : 1, most = (keys + 127) / 128;
-    plan.splits = (uint32_t)(wanted < most ? wanted : most);
+    const uint64_t whole = ((uint64_t)a.q_rows * group / (16 * plan.blocks) + a.documents) * a.kv_heads, units = compute_units;
+    if (plan.blocks == PAGED_CHUNK_BLOCKS) {
+        // Equal shares of keys, so that the chip is filled three times over by what
+        // the host knows of the lengths: 8 documents, four of 1024 queries over 1641
+        // to 6837 keys (544 workgroups), capped, bf16: 264 us, unsplit 300; but four
+        // of equal length 380 and 348. Small shares cost more sums than they fill
+        // compute units: 300 queries of three documents over 600 keys 31 us in shares
+        // of 256, 39 in 128; 100 of one over 2000 24 and 21.
+        uint64_t share = keys;
+        if (whole < 4 * units) share = (whole * keys + 3 * units - 1) / (3 * units);
+        const uint64_t step = share >= 512 ? 512 : whole <= units / 4 ? 128 : 256;
+        plan.share = (uint32_t)((share + step - 1) / step * step);
+        if (plan.share < step) plan.share = (uint32_t)step;
+        plan.splits = (uint32_t)((keys + plan.share - 1) / plan.share);
+    } else {
+        // Even shares of each document: four workgroups a compute unit (32 tokens over
+        // 3300 to 16153 keys in codes, 8 key heads of 128: 108 us; two 120, eight 121).
+        const uint64_t wanted = whole < 4 * units ? (4 * units + whole - 1) / whole : 1, most = (keys + 127) / 128;
+        plan.splits = (uint32_t)(wanted < most ? wanted : most);
+    }
     if (plan.splits < 1) plan.splits = 1;
     if (plan.splits > 1) {
         plan.partial_bytes = rounded(plan.splits * places * plan.tile_dim * sizeof(float));
-        plan.stats_bytes = rounded(plan.splits * places * 2 * sizeof(float));
+        plan.stats_bytes = rounded(plan.splits * places * 4 * sizeof(float));
     }
     return plan;
 }
@@ -33,6 +50,7 @@ PagedPlan plan_paged(const bl_paged_attention_args &a, uint32_t compute_units) {
 hipError_t launch_paged(const bl_paged_attention_args &a, const PagedPlan &plan, hipStream_t s) {
     PagedParams p{};
     p.a = a;
+    p.share = plan.share;
     p.splits = plan.splits;
     p.page_magic = (uint32_t)(((1ull << 32) + a.cache.page_rows - 1) / a.cache.page_rows);
     p.partial = (float *)a.workspace;
