@@ -19,6 +19,7 @@ struct HeadsGeometry {
     uint32_t head_groups;  // a power of two
     uint32_t rows;         // 256 / (lanes * head_groups): rows a workgroup holds at once
     uint32_t first;        // the launch's first row
+    uint32_t span;         // of the backward: a workgroup's rows, a multiple of `rows`
 };
 
 // Units of a thread: heads of 256 channels with single elements have 255.
@@ -34,7 +35,7 @@ inline HeadsGeometry heads_geometry(uint32_t vec, uint32_t pairs, uint32_t head_
     g.lanes = least_lanes;
     while (g.lanes * up < g.units) g.lanes *= 2;
     g.head_groups = 1;
-    while (2 * g.head_groups * g.lanes <= 256 && g.head_groups < heads && rows < workgroups * (256 / (g.lanes * g.head_groups))) g.head_groups *= 2;
+    while (2 * g.head_groups * g.lanes <= 256 && 2 * g.head_groups <= heads && rows < workgroups * (256 / (g.lanes * g.head_groups))) g.head_groups *= 2;
     g.rows = 256 / (g.lanes * g.head_groups);
     return g;
 }
@@ -215,6 +216,13 @@ template <int VEC, typename F> struct Turn {
         }
     }
 };
+
+// A register that the compiler takes for new: what is loaded by way of it is not
+// kept over a loop's turns.
+__device__ __forceinline__ uint32_t fresh(uint32_t v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
 
 __device__ __forceinline__ void sine_of(double t, float &si, float &co) { sincospif(2.0f * (float)t, &si, &co); }
 __device__ __forceinline__ void sine_of(double t, double &si, double &co) { sincospi(2.0 * t, &si, &co); }

@@ -45,26 +45,61 @@ __global__ __launch_bounds__(256) void forward_kernel(HeadsParams p, HeadsGeomet
     forward_heads<T, VEC>(p, g, seat, row, p.k_in, p.k_out, p.k_heads, p.k_gamma, c, turn);
 }
 
+// What a thread reads of two heads' channels, as they lie in memory.
+template <typename T, int VEC> struct Raw {
+    static constexpr int UP = UNITS<VEC>;
+    typedef T V __attribute__((ext_vector_type(VEC)));
+    V first[UP], second[UP];
+    __device__ __forceinline__ void load(const T *head, const Chunk<VEC> (&c)[UP]) {
+#pragma unroll
+        for (int k = 0; k < UP; k++) {
+            first[k] = second[k] = V{};
+            if (c[k].there) first[k] = *(const V *)(head + c[k].c0);
+            if (c[k].pair) second[k] = *(const V *)(head + c[k].c1);
+        }
+    }
+    __device__ __forceinline__ void to(Channels<VEC, float> &x) const {
+#pragma unroll
+        for (int k = 0; k < UP; k++)
+#pragma unroll
+            for (int e = 0; e < VEC; e++) x.v[k][e] = (float)first[k][e], x.v[k][VEC + e] = (float)second[k][e];
+    }
+};
+
+// `sines`: LDS, the row's; the weights lie there too, as they were read, and
+// neither is kept in registers over the heads: with them a SIMD has room for five
+// waves instead of three.
 template <typename T, int VEC>
 __device__ __forceinline__ void backward_heads(const HeadsParams &p, const HeadsGeometry &g, const Seat &seat, uint64_t row, const bl_heads &in, const bl_heads &d_out,
-                                               const bl_heads &d_in, uint32_t heads, const void *gamma, const Chunk<VEC> (&c)[UNITS<VEC>],
-                                               const Turn<VEC, float> &turn, Channels<VEC, float> &d_gamma) {
+                                               const bl_heads &d_in, uint32_t heads, const float *weights, const Chunk<VEC> (&c)[UNITS<VEC>],
+                                               const float *cosines, const float *sines, Channels<VEC, float> &d_gamma) {
     if (seat.group >= heads) return;
-    const Channels<VEC, float> weights = weights_of<VEC, float, T>(gamma, c);
     const T *src = (const T *)in.data + row * in.row_stride, *dy = (const T *)d_out.data + row * d_out.row_stride;
     T *dst = (T *)d_in.data + row * d_in.row_stride;
     const float each = 1.0f / (float)p.head_dim;
+    Raw<T, VEC> x, y;
+    x.load(src + (uint64_t)seat.group * in.head_stride, c);
+    y.load(dy + (uint64_t)seat.group * d_out.head_stride, c);
     for (uint32_t h = seat.group; h < heads; h += g.head_groups) {
         Channels<VEC, float> n, z;
-        n.load(src + (uint64_t)h * in.head_stride, c);
-        z.load(dy + (uint64_t)h * d_out.head_stride, c);
+        x.to(n);
+        y.to(z);
+        if (h + g.head_groups < heads) {  // the next head's on their way
+            x.load(src + (uint64_t)(h + g.head_groups) * in.head_stride, c);
+            y.load(dy + (uint64_t)(h + g.head_groups) * d_out.head_stride, c);
+        }
         const float rstd = n.normalise(p.norm, p.epsilon, p.head_dim, g.lanes, c);
+        Turn<VEC, float> turn;
+        const uint32_t at = fresh(0);
+        turn.load(cosines + at, sines + at, c);
         turn.apply(z, p.table.layout, -1.0f, c);
 #pragma unroll
         for (int k = 0; k < UNITS<VEC>; k++)
 #pragma unroll
             for (int e = 0; e < 2 * VEC; e++) d_gamma.v[k][e] += z.v[k][e] * n.v[k][e];
-        z.times(weights);
+        Channels<VEC, float> w;
+        w.load(weights + fresh(0), c);
+        z.times(w);
         const float along = z.dot(n, g.lanes) * each;
         if (p.norm == BL_HEAD_NORM_CENTRED) z.less(z.sum(g.lanes) * each, c);
 #pragma unroll
@@ -98,38 +133,46 @@ template <typename T, int VEC>
 __global__ __launch_bounds__(256) void backward_kernel(HeadsParams p, HeadsGeometry g) {
     constexpr int UP = UNITS<VEC>;
     __shared__ __attribute__((aligned(16))) float lds[2][256 * UP * VEC];  // cosines, sines; in the end the weights' sums
+    __shared__ __attribute__((aligned(16))) float weights[2][BL_HEAD_NORM_MAX_HEAD_DIM];
     const Seat seat(g);
     Chunk<VEC> c[UP];
     chunks_of<VEC>(g, p.table, seat.lane, c);
+    for (uint32_t n = threadIdx.x; n < p.head_dim; n += 256) {
+        weights[0][n] = p.q_gamma ? (float)((const T *)p.q_gamma)[n] : 1.0f;
+        weights[1][n] = p.k_gamma ? (float)((const T *)p.k_gamma)[n] : 1.0f;
+    }
     Channels<VEC, float> d_q = {}, d_k = {};
-    for (uint64_t first = (uint64_t)blockIdx.x * g.rows; first < p.rows; first += (uint64_t)p.groups * g.rows) {
+    // The sines of as many rows at once as there is room for.
+    const uint32_t room = p.table.pairs ? (256 * UP * VEC / p.table.pairs) / g.rows * g.rows : g.span, batch = min(room, g.span);
+    const uint64_t begin = (uint64_t)blockIdx.x * g.span, end = min(begin + g.span, (uint64_t)p.rows);
+    for (uint64_t first = begin; first < end; first += batch) {
         __syncthreads();  // the last rows' sines have been read
-        make_sines(p.table, g.rows, first, p.rows, lds[0], lds[1], [&](uint32_t, uint64_t r, uint32_t axis) { return p.positions[r * p.table.axes + axis]; });
+        make_sines(p.table, batch, first, end, lds[0], lds[1], [&](uint32_t, uint64_t r, uint32_t axis) { return p.positions[r * p.table.axes + axis]; });
         __syncthreads();
-        const uint64_t row = first + seat.slot;
-        if (row >= p.rows) continue;
-        Turn<VEC, float> turn;
-        turn.load(lds[0] + seat.slot * p.table.pairs, lds[1] + seat.slot * p.table.pairs, c);
-        backward_heads<T, VEC>(p, g, seat, row, p.q_in, p.dq_out, p.dq_in, p.q_heads, p.q_gamma, c, turn, d_q);
-        backward_heads<T, VEC>(p, g, seat, row, p.k_in, p.dk_out, p.dk_in, p.k_heads, p.k_gamma, c, turn, d_k);
+        for (uint64_t row = first + seat.slot; row < min(first + batch, end); row += g.rows) {
+            const float *const cosines = lds[0] + (uint32_t)(row - first) * p.table.pairs, *const sines = lds[1] + (uint32_t)(row - first) * p.table.pairs;
+            backward_heads<T, VEC>(p, g, seat, row, p.q_in, p.dq_out, p.dq_in, p.q_heads, weights[0], c, cosines, sines, d_q);
+            backward_heads<T, VEC>(p, g, seat, row, p.k_in, p.dk_out, p.dk_in, p.k_heads, weights[1], c, cosines, sines, d_k);
+        }
     }
     float *out = p.partial + (uint64_t)blockIdx.x * 2 * p.head_dim;
     sum_seats<VEC>(g, p.table.pairs, p.table.layout, d_q, lds[0], out);
     sum_seats<VEC>(g, p.table.pairs, p.table.layout, d_k, lds[0], out + p.head_dim);
 }
 
-// The workgroups' sums added: 16 channels a workgroup, 16 threads a channel.
-__global__ __launch_bounds__(256) void weights_kernel(HeadsParams p) {
-    __shared__ float lds[16][17];
+// The workgroups' sums added: 16 channels a workgroup, 64 threads a channel.
+__global__ __launch_bounds__(1024) void weights_kernel(HeadsParams p) {
+    __shared__ float lds[64][17];
     const uint32_t c = blockIdx.x * 16 + threadIdx.x % 16, part = threadIdx.x / 16, all = 2 * p.head_dim;
     float s = 0.0f;
     if (c < all)
-        for (uint32_t n = part; n < p.groups; n += 16) s += p.partial[(uint64_t)n * all + c];
+#pragma unroll 8
+        for (uint32_t n = part; n < p.groups; n += 64) s += p.partial[(uint64_t)n * all + c];
     lds[part][threadIdx.x % 16] = s;
     __syncthreads();
     if (part || c >= all) return;
 #pragma unroll
-    for (int n = 1; n < 16; n++) s += lds[n][threadIdx.x];
+    for (int n = 1; n < 64; n++) s += lds[n][threadIdx.x];
     if (c < p.head_dim) {
         if (p.d_q_gamma) p.d_q_gamma[c] = s;
     } else if (p.d_k_gamma) {
@@ -153,13 +196,22 @@ hipError_t forward(const HeadsParams &p, uint32_t compute_units, hipStream_t s) 
 template <typename T, int VEC>
 hipError_t backward(const HeadsParams &q, hipStream_t s) {
     HeadsParams p = q;
-    const HeadsGeometry g = heads_geometry(VEC, p.table.pairs, p.head_dim, p.q_heads > p.k_heads ? p.q_heads : p.k_heads, p.rows, 1, p.groups);
-    // No more workgroups than it takes for the largest share of the rows' blocks.
-    const uint32_t blocks = (uint32_t)(((uint64_t)p.rows + g.rows - 1) / g.rows), share = blocks ? (blocks + p.groups - 1) / p.groups : 1;
-    p.groups = blocks ? (blocks + share - 1) / share : 1;
+    // As many heads at once as leave a workgroup the fewest turns: 32768 rows of 16 +
+    // 4 heads go 4 at a time, 4099 of 9 + 3 two.
+    HeadsGeometry g = heads_geometry(VEC, p.table.pairs, p.head_dim, 1, p.rows, 1, 0);
+    const uint64_t each = ((uint64_t)p.rows + p.groups - 1) / p.groups;
+    uint64_t fewest = ~0ull;
+    for (uint32_t at_once = 1; at_once * g.lanes <= 256 && at_once < 2 * (p.q_heads > p.k_heads ? p.q_heads : p.k_heads); at_once *= 2) {
+        const uint32_t rows = 256 / (g.lanes * at_once);
+        const uint64_t turns = ((p.q_heads + at_once - 1) / at_once + (p.k_heads + at_once - 1) / at_once) * ((each + rows - 1) / rows);
+        if (turns <= fewest) fewest = turns, g.head_groups = at_once, g.rows = rows;
+    }
+    g.span = (uint32_t)((each + g.rows - 1) / g.rows * g.rows);
+    if (g.span == 0) g.span = g.rows;
+    p.groups = p.rows ? (p.rows + g.span - 1) / g.span : 1;
     const hipError_t e = run_kernel(backward_kernel<T, VEC>, p.groups, 256, s, p, g);
     if (e != hipSuccess || (!p.d_q_gamma && !p.d_k_gamma)) return e;
-    return run_kernel(weights_kernel, (2 * p.head_dim + 15) / 16, 256, s, p);
+    return run_kernel(weights_kernel, (2 * p.head_dim + 15) / 16, 1024, s, p);
 }
 
 }  // namespace

@@ -93,7 +93,7 @@ struct HeadsParams {
     uint32_t groups;         // workgroups that walk the rows of the backward
     uint32_t vec;            // elements of an access: 16 bytes, 8 or one element, as everything is aligned
 };
-constexpr uint32_t HEADS_BACKWARD_GROUPS = 4;  // a compute unit
+constexpr uint32_t HEADS_BACKWARD_GROUPS = 3;  // a compute unit: as many as there is room for with 16-byte accesses of 16-bit types
 hipError_t launch_heads_forward(const HeadsParams &p, uint32_t dtype, uint32_t compute_units, hipStream_t s);
 hipError_t launch_heads_backward(const HeadsParams &p, uint32_t dtype, uint32_t compute_units, hipStream_t s);
 
