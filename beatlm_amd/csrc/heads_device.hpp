@@ -164,6 +164,27 @@ template <int VEC, typename F> struct Channels {
     }
 };
 
+// What a thread reads of a head, as it lies in memory: the next head's, on its way.
+template <typename T, int VEC> struct Raw {
+    static constexpr int UP = UNITS<VEC>;
+    typedef T V __attribute__((ext_vector_type(VEC)));
+    V first[UP], second[UP];
+    __device__ __forceinline__ void load(const T *head, const Chunk<VEC> (&c)[UP]) {
+#pragma unroll
+        for (int k = 0; k < UP; k++) {
+            first[k] = second[k] = V{};
+            if (c[k].there) first[k] = *(const V *)(head + c[k].c0);
+            if (c[k].pair) second[k] = *(const V *)(head + c[k].c1);
+        }
+    }
+    template <typename F> __device__ __forceinline__ void to(Channels<VEC, F> &x) const {
+#pragma unroll
+        for (int k = 0; k < UP; k++)
+#pragma unroll
+            for (int e = 0; e < VEC; e++) x.v[k][e] = (F)(float)first[k][e], x.v[k][VEC + e] = (F)(float)second[k][e];
+    }
+};
+
 // The weights: ones without any.
 template <int VEC, typename F, typename T>
 __device__ __forceinline__ Channels<VEC, F> weights_of(const void *gamma, const Chunk<VEC> (&c)[UNITS<VEC>]) {
@@ -226,6 +247,29 @@ __device__ __forceinline__ uint32_t fresh(uint32_t v) {
 
 __device__ __forceinline__ void sine_of(double t, float &si, float &co) { sincospif(2.0f * (float)t, &si, &co); }
 __device__ __forceinline__ void sine_of(double t, double &si, double &co) { sincospi(2.0 * t, &si, &co); }
+
+// A head's rotation and weights from LDS, not kept in registers over the heads.
+template <int VEC, typename F, typename S>
+__device__ __forceinline__ void turn_by(Channels<VEC, F> &x, const S *cosines, const S *sines, uint32_t layout, F sign, const Chunk<VEC> (&c)[UNITS<VEC>]) {
+    Turn<VEC, F> turn;
+    const uint32_t at = fresh(0);
+    turn.load(cosines + at, sines + at, c);
+    turn.apply(x, layout, sign, c);
+}
+template <int VEC, typename F>
+__device__ __forceinline__ void weigh_by(Channels<VEC, F> &x, const float *weights, const Chunk<VEC> (&c)[UNITS<VEC>]) {
+    Channels<VEC, F> w;
+    w.load(weights + fresh(0), c);
+    x.times(w);
+}
+// Both tensors' weights to LDS, ones without any.
+template <typename T, int MOST>
+__device__ __forceinline__ void put_weights(const HeadsParams &p, float (&weights)[2][MOST]) {
+    for (uint32_t n = threadIdx.x; n < p.head_dim; n += 256) {
+        weights[0][n] = p.q_gamma ? (float)((const T *)p.q_gamma)[n] : 1.0f;
+        weights[1][n] = p.k_gamma ? (float)((const T *)p.k_gamma)[n] : 1.0f;
+    }
+}
 
 // The sines and cosines of `rows` rows, the first of them `first`, [rows][pairs];
 // position(slot, row, axis) of rows up to `last`. Angles are reduced in 64 bits.

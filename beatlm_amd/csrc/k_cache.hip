@@ -84,9 +84,8 @@ __device__ __forceinline__ float rounded_once(double v) {
 }
 
 // 8 channels of a group that the lane's quad shares, to their codes, and from
-// the quad's first lane the group's step and low. Both round once from f32, and
-// codes are found in 64 bits, where a value's distance to low is exact: a tie is
-// one on every path.
+// the quad's first lane the group's step and low. A value's distance to low is
+// exact in 64 bits: a tie between two codes is one on every path.
 __device__ __forceinline__ void store_codes(const float (&x)[8], char *row, uint32_t head_dim, uint32_t chunk) {
     float least = x[0], most = x[0], bad = 0.0f;
 #pragma unroll
@@ -99,13 +98,26 @@ __device__ __forceinline__ void store_codes(const float (&x)[8], char *row, uint
     most = -quad_min(-most);
     bad = -quad_min(-bad);
     const uint32_t low_bits = half_bits(least), step_bits = bad != 0.0f ? 0x7e00u : half_bits(rounded_once(((double)most - (double)least) / 15.0));
-    const double low = (float)__builtin_bit_cast(_Float16, (uint16_t)low_bits), step = (float)__builtin_bit_cast(_Float16, (uint16_t)step_bits);
-    uint32_t codes = 0;
+    const float low = (float)__builtin_bit_cast(_Float16, (uint16_t)low_bits), step = (float)__builtin_bit_cast(_Float16, (uint16_t)step_bits);
+    // In f32 a code's place is off by some 2^-20: only where that might cross the
+    // middle between two codes is it found in 64 bits. A step of zero or NaN:
+    // whatever the code, the value is low or NaN.
+    const float per = __builtin_amdgcn_rcpf(step);
+    uint32_t codes = 0, close = 0;
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-        // A step of zero or NaN: whatever the code, the value is low or NaN.
-        const double code = step > 0.0 ? fmin(fmax(rint(((double)x[e] - low) / step), 0.0), 15.0) : 0.0;
-        codes |= (uint32_t)code << (e / 2 * 4 + e % 2 * 16);
+        const float place = (x[e] - low) * per, code = rintf(place);
+        close |= (fabsf(place - code) > 0.4999f ? 1u : 0u) << e;
+        codes |= (step > 0.0f ? (uint32_t)fminf(fmaxf(code, 0.0f), 15.0f) : 0u) << (e / 2 * 4 + e % 2 * 16);
+    }
+    if (close && step > 0.0f) {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            if (close >> e & 1) {
+                const double code = fmin(fmax(rint(((double)x[e] - (double)low) / (double)step), 0.0), 15.0);
+                const int at = e / 2 * 4 + e % 2 * 16;
+                codes = (codes & ~(15u << at)) | (uint32_t)code << at;
+            }
     }
     *(uint32_t *)(row + chunk * 4) = codes;
     if (chunk % 4 == 0) *(uint32_t *)(row + head_dim / 2 + chunk) = step_bits | low_bits << 16;
@@ -126,14 +138,25 @@ __device__ __forceinline__ void load8(const T *p, float (&x)[8]) {
 
 template <typename T, int VEC, bool INT4>
 __global__ __launch_bounds__(256) void append_kernel(AppendParams p, HeadsGeometry g) {
-    constexpr int UP = UNITS<VEC>, HELD = 256 * UP * VEC;
+    constexpr int UP = UNITS<VEC>;
     typedef std::conditional_t<INT4, double, float> F;
-    __shared__ __attribute__((aligned(16))) F cosines[HELD], sines[HELD];
-    __shared__ __attribute__((aligned(16))) float staged[INT4 ? 2 * HELD : 1];  // a head's channels for each of the seats' lanes
+    extern __shared__ __attribute__((aligned(16))) char turns[];  // of the rows' pairs, as many as there are
+    F *const cosines = (F *)turns, *const sines = cosines + g.rows * p.h.table.pairs;
+    __shared__ __attribute__((aligned(16))) float staged[INT4 ? 2 * 256 * UP * VEC : 1];  // a head's channels for each of the seats' lanes
     __shared__ Home homes[256];
+    __shared__ __attribute__((aligned(16))) float weights[2][BL_ATTENTION_MAX_HEAD_DIM];
     const HeadsParams &a = p.h;
     const Seat seat(g);
     const uint64_t first = g.first + (uint64_t)blockIdx.x * g.rows, row = first + seat.slot;
+    Chunk<VEC> c[UP];
+    chunks_of<VEC>(g, a.table, seat.lane, c);
+    // The first heads are on their way while the rows' homes are looked up.
+    const T *const q = (const T *)a.q_in.data + row * a.q_in.row_stride, *const k = (const T *)a.k_in.data + row * a.k_in.row_stride;
+    Raw<T, VEC> next_q, next_k;
+    const bool has_q = row < a.rows && seat.group < a.q_heads, has_k = row < a.rows && seat.group < a.k_heads;
+    if (has_q) next_q.load(q + (uint64_t)seat.group * a.q_in.head_stride, c);
+    if (has_k) next_k.load(k + (uint64_t)seat.group * a.k_in.head_stride, c);
+    if (a.norm != BL_HEAD_NORM_NONE) put_weights<T>(a, weights);
     find_homes(p.q_offsets, (int)p.documents, g.rows, first, a.rows, homes,
                [&](int d, int64_t i, int64_t n) { return page_of(p.cache, d, (int64_t)p.cache.lengths[d] - n + i); });
     __syncthreads();
@@ -144,40 +167,33 @@ __global__ __launch_bounds__(256) void append_kernel(AppendParams p, HeadsGeomet
     if (row >= a.rows) return;
     const Home home = homes[seat.slot];
     if (home.place == NOBODY) return;
-    Chunk<VEC> c[UP];
-    chunks_of<VEC>(g, a.table, seat.lane, c);
     const F *const co = cosines + seat.slot * a.table.pairs, *const si = sines + seat.slot * a.table.pairs;
-    if (seat.group < a.q_heads) {
-        Turn<VEC, float> turn;
-        turn.load(co, si, c);
-        const Channels<VEC, float> weights = weights_of<VEC, float, T>(a.q_gamma, c);
-        const T *src = (const T *)a.q_in.data + row * a.q_in.row_stride;
+    if (has_q) {
         T *dst = (T *)a.q_out.data + row * a.q_out.row_stride;
         for (uint32_t h = seat.group; h < a.q_heads; h += g.head_groups) {
             Channels<VEC, float> x;
-            x.load(src + (uint64_t)h * a.q_in.head_stride, c);
+            next_q.to(x);
+            if (h + g.head_groups < a.q_heads) next_q.load(q + (uint64_t)(h + g.head_groups) * a.q_in.head_stride, c);
             if (a.norm != BL_HEAD_NORM_NONE) {
                 x.normalise(a.norm, a.epsilon, a.head_dim, g.lanes, c);
-                x.times(weights);
+                weigh_by<VEC>(x, weights[0], c);
             }
-            turn.apply(x, a.table.layout, 1.0f, c);
+            turn_by<VEC>(x, co, si, a.table.layout, 1.0f, c);
             x.store(dst + (uint64_t)h * a.q_out.head_stride, c);
         }
     }
-    if (home.page < 0 || seat.group >= a.k_heads) return;
-    Turn<VEC, F> turn;
-    turn.load(co, si, c);
-    const Channels<VEC, F> weights = weights_of<VEC, F, T>(a.k_gamma, c);
-    const T *k = (const T *)a.k_in.data + row * a.k_in.row_stride, *v = (const T *)p.v_in.data + row * p.v_in.row_stride;
+    if (home.page < 0 || !has_k) return;
+    const T *const v = (const T *)p.v_in.data + row * p.v_in.row_stride;
     char *const k_row = row_of(p.cache.k, home), *const v_row = row_of(p.cache.v, home);
     for (uint32_t h = seat.group; h < a.k_heads; h += g.head_groups) {
         Channels<VEC, F> x;
-        x.load(k + (uint64_t)h * a.k_in.head_stride, c);
+        next_k.to(x);
+        if (h + g.head_groups < a.k_heads) next_k.load(k + (uint64_t)(h + g.head_groups) * a.k_in.head_stride, c);
         if (a.norm != BL_HEAD_NORM_NONE) {
             x.normalise(a.norm, a.epsilon, a.head_dim, g.lanes, c);
-            x.times(weights);
+            weigh_by<VEC>(x, weights[1], c);
         }
-        turn.apply(x, a.table.layout, F(1), c);
+        turn_by<VEC>(x, co, si, a.table.layout, F(1), c);
         const T *value = v + (uint64_t)h * p.v_in.head_stride;
         char *const to_k = k_row + (uint64_t)h * p.cache.k.head_stride, *const to_v = v_row + (uint64_t)h * p.cache.v.head_stride;
         if constexpr (INT4) {
@@ -269,9 +285,11 @@ template <typename T, int VEC>
 hipError_t append(const AppendParams &p, uint32_t compute_units, hipStream_t s) {
     const HeadsParams &a = p.h;
     const bool int4 = p.cache.kind == BL_CACHE_INT4;
-    HeadsGeometry g = heads_geometry(VEC, a.table.pairs, a.head_dim, a.q_heads > a.k_heads ? a.q_heads : a.k_heads, a.rows, int4 ? 4 : 1, 2ull * compute_units);
+    HeadsGeometry g = heads_geometry(VEC, a.table.pairs, a.head_dim, a.q_heads > a.k_heads ? a.q_heads : a.k_heads, a.rows, int4 ? 4 : 1, 4ull * compute_units);
     return in_parts(g, a.rows, [&](uint32_t grid) {
-        return int4 ? run_kernel(append_kernel<T, VEC, true>, grid, 256, s, p, g) : run_kernel(append_kernel<T, VEC, false>, grid, 256, s, p, g);
+        const uint32_t held = 2 * g.rows * a.table.pairs;
+        return int4 ? run_kernel_with(held * sizeof(double), append_kernel<T, VEC, true>, grid, 256, s, p, g)
+                    : run_kernel_with(held * sizeof(float), append_kernel<T, VEC, false>, grid, 256, s, p, g);
     });
 }
 

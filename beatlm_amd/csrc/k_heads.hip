@@ -45,27 +45,6 @@ __global__ __launch_bounds__(256) void forward_kernel(HeadsParams p, HeadsGeomet
     forward_heads<T, VEC>(p, g, seat, row, p.k_in, p.k_out, p.k_heads, p.k_gamma, c, turn);
 }
 
-// What a thread reads of two heads' channels, as they lie in memory.
-template <typename T, int VEC> struct Raw {
-    static constexpr int UP = UNITS<VEC>;
-    typedef T V __attribute__((ext_vector_type(VEC)));
-    V first[UP], second[UP];
-    __device__ __forceinline__ void load(const T *head, const Chunk<VEC> (&c)[UP]) {
-#pragma unroll
-        for (int k = 0; k < UP; k++) {
-            first[k] = second[k] = V{};
-            if (c[k].there) first[k] = *(const V *)(head + c[k].c0);
-            if (c[k].pair) second[k] = *(const V *)(head + c[k].c1);
-        }
-    }
-    __device__ __forceinline__ void to(Channels<VEC, float> &x) const {
-#pragma unroll
-        for (int k = 0; k < UP; k++)
-#pragma unroll
-            for (int e = 0; e < VEC; e++) x.v[k][e] = (float)first[k][e], x.v[k][VEC + e] = (float)second[k][e];
-    }
-};
-
 // `sines`: LDS, the row's; the weights lie there too, as they were read, and
 // neither is kept in registers over the heads: with them a SIMD has room for five
 // waves instead of three.
@@ -89,17 +68,12 @@ __device__ __forceinline__ void backward_heads(const HeadsParams &p, const Heads
             y.load(dy + (uint64_t)(h + g.head_groups) * d_out.head_stride, c);
         }
         const float rstd = n.normalise(p.norm, p.epsilon, p.head_dim, g.lanes, c);
-        Turn<VEC, float> turn;
-        const uint32_t at = fresh(0);
-        turn.load(cosines + at, sines + at, c);
-        turn.apply(z, p.table.layout, -1.0f, c);
+        turn_by<VEC>(z, cosines, sines, p.table.layout, -1.0f, c);
 #pragma unroll
         for (int k = 0; k < UNITS<VEC>; k++)
 #pragma unroll
             for (int e = 0; e < 2 * VEC; e++) d_gamma.v[k][e] += z.v[k][e] * n.v[k][e];
-        Channels<VEC, float> w;
-        w.load(weights + fresh(0), c);
-        z.times(w);
+        weigh_by<VEC>(z, weights, c);
         const float along = z.dot(n, g.lanes) * each;
         if (p.norm == BL_HEAD_NORM_CENTRED) z.less(z.sum(g.lanes) * each, c);
 #pragma unroll
@@ -137,10 +111,7 @@ __global__ __launch_bounds__(256) void backward_kernel(HeadsParams p, HeadsGeome
     const Seat seat(g);
     Chunk<VEC> c[UP];
     chunks_of<VEC>(g, p.table, seat.lane, c);
-    for (uint32_t n = threadIdx.x; n < p.head_dim; n += 256) {
-        weights[0][n] = p.q_gamma ? (float)((const T *)p.q_gamma)[n] : 1.0f;
-        weights[1][n] = p.k_gamma ? (float)((const T *)p.k_gamma)[n] : 1.0f;
-    }
+    put_weights<T>(p, weights);
     Channels<VEC, float> d_q = {}, d_k = {};
     // The sines of as many rows at once as there is room for.
     const uint32_t room = p.table.pairs ? (256 * UP * VEC / p.table.pairs) / g.rows * g.rows : g.span, batch = min(room, g.span);

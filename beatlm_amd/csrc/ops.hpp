@@ -114,6 +114,7 @@ hipError_t launch_cache_read(const bl_cache_read_args &a, uint32_t compute_units
 constexpr uint32_t PAGED_CHUNK_BLOCKS = 8;
 struct PagedPlan {
     uint32_t blocks;    // of 16 (query, head of a group) places in a workgroup: 1, 2 or PAGED_CHUNK_BLOCKS
+    uint32_t waves;     // of a workgroup, 4 or 8: without splits, of few places
     uint32_t share;     // of chunks: keys of a workgroup, from the first that its places see
     uint32_t splits;    // workgroups that share a document's keys; of chunks the longest one's, and the last takes what is left of a longer one
     uint32_t tile_dim;  // channels of the kernels' tiles: 64 or 128

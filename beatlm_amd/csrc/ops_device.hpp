@@ -27,6 +27,13 @@ __device__ __forceinline__ float sum_xor16(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// The same with `lds` bytes of LDS beside what the kernel declares.
+template <typename... P>
+hipError_t run_kernel_with(uint32_t lds, void (*kernel)(P...), dim3 grid, uint32_t threads, hipStream_t s, const P &...params) {
+    void *args[] = {(void *)&params...};
+    return hipLaunchKernel((const void *)kernel, grid, dim3(threads), args, lds, s);
+}
+
 // VEC elements at p (16-byte aligned when VEC > 1) as f32.
 template <typename T, int VEC>
 __device__ __forceinline__ void load_vec(const T *p, float (&v)[VEC]) {

@@ -11,13 +11,19 @@ uint64_t rounded(uint64_t bytes) { return (bytes + 255) / 256 * 256; }
 
 PagedPlan plan_paged(const bl_paged_attention_args &a, uint32_t compute_units) {
     PagedPlan plan{};
+    plan.waves = 4;
     plan.tile_dim = a.head_dim <= 64 ? 64 : 128;
     const uint64_t group = a.q_heads / a.kv_heads, places = (uint64_t)a.q_rows * a.q_heads;
     const uint64_t average = ((uint64_t)a.q_rows * group + a.documents - 1) / a.documents;
-    plan.blocks = average <= 16 ? 1 : average <= 32 ? 2 : PAGED_CHUNK_BLOCKS;
     const uint64_t table = (uint64_t)a.cache.max_pages * a.cache.page_rows;
     uint64_t keys = a.max_keys && a.max_keys < table ? a.max_keys : table;
     if (a.window && (uint64_t)a.window + a.q_rows < keys) keys = (uint64_t)a.window + a.q_rows;
+    // 16 or 32 places a workgroup, whose waves share its keys, or 128, which share a
+    // tile of them. Over long caches two workgroups of 32 keep more loads under way
+    // (9 documents of 40 places over 3450 to 11500 keys, heads of 64, f16: 27 us, 128
+    // places 35; in codes 31 and 39); over 2049 keys they take 17 us and 16, and 96
+    // places 27 and 20.
+    plan.blocks = average <= 16 ? 1 : average <= 32 || (average <= 64 && keys >= 4096) ? 2 : PAGED_CHUNK_BLOCKS;
     // Workgroups without splits, and a last, partial one a document.
     const uint64_t whole = ((uint64_t)a.q_rows * group / (16 * plan.blocks) + a.documents) * a.kv_heads, units = compute_units;
     if (plan.blocks == PAGED_CHUNK_BLOCKS) {
@@ -38,6 +44,11 @@ PagedPlan plan_paged(const bl_paged_attention_args &a, uint32_t compute_units) {
         // 3300 to 16153 keys in codes, 8 key heads of 128: 108 us; two 120, eight 121).
         const uint64_t wanted = whole < 4 * units ? (4 * units + whole - 1) / whole : 1, most = (keys + 127) / 128;
         plan.splits = (uint32_t)(wanted < most ? wanted : most);
+        // Few keys: eight waves a workgroup, one or two steps each, and no second launch
+        // to join splits (one token, 12 heads of 64: over 300 keys 6.8 us, split 9.3;
+        // over 700 9.2 and 10.0, over 1500 13.0 and 9.4; heads of 128 8.5 and 10.0, 12.1
+        // and 10.4, 18.8 and 11.1).
+        if (plan.blocks == 1 && keys <= 512 && whole <= units) plan.waves = 8, plan.splits = 1;
     }
     if (plan.splits < 1) plan.splits = 1;
     if (plan.splits > 1) {
