@@ -313,6 +313,22 @@ def test_paged_attention(gpu, dtype, kind, case):
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("lengths,queries,q_heads,kv_heads,d,max_keys", [
+    ([5000, 1203], [1, 1], 8, 2, 128, 0), ([4500, 9000], [5, 5], 8, 1, 64, 9000), ([4500, 100], [8, 8], 6, 1, 96, 200), ([3000], [200], 4, 2, 128, 0),
+    ([3000, 2500], [150, 1], 4, 4, 64, 700), ([512], [1], 4, 4, 128, 512), ([513], [1], 4, 4, 64, 513),
+])
+def test_splits_and_long_caches(gpu, dtype, kind, lengths, queries, q_heads, kv_heads, d, max_keys):
+    """Keys split over workgroups, each kernel's form, and documents longer than the host said."""
+    cache = Cache(lengths, dtype, kind, kv_heads, d, 64)
+    t = Queries(cache, queries, dtype, q_heads)
+    ops.paged_attention(gpu, t.args(gpu, max_keys))
+    out, out_tol, lse, lse_tol = t.reference()
+    assert_within(t.out, out, out_tol, "out")
+    assert_within(t.lse, lse, lse_tol, "lse")
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("kind", list(KINDS))
 @pytest.mark.parametrize("options", [dict(mask="causal", window=30), dict(mask="causal"), dict(mask="none")])
 @pytest.mark.parametrize("queries", [1, 6, 50])
 def test_pages_that_are_not_there_and_keys_of_anything(gpu, dtype, kind, options, queries):
@@ -430,6 +446,29 @@ def test_wrong_offsets_and_lengths_stay_inside(gpu, dtype, kind, offsets):
 
 
 @pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("queries", [1, 40])
+def test_what_the_workspace_held_does_not_count(gpu, kind, queries):
+    """Counts and maxima of earlier calls, here large numbers, with right offsets and with wrong ones."""
+    cache = Cache([900, 70, 300], "bf16", kind, 2, 64, 16)
+    t = Queries(cache, [queries, 1, queries], "bf16", 8)
+    a = t.args(gpu)
+    n = a.workspace_bytes
+    assert n > 0
+    space = torch.full((n // 4 + 128,), 1e9, device="cuda")
+    a.workspace = space.data_ptr() + 256
+    ops.paged_attention(gpu, a)
+    out, out_tol, lse, lse_tol = t.reference()
+    assert_within(t.out, out, out_tol, "out")
+    assert_within(t.lse, lse, lse_tol, "lse")
+    for offsets in ([0, queries, 0, 2 * queries + 1], [1, 0, 0, 2 * queries]):
+        t.offsets.copy_(torch.tensor(offsets))
+        space.fill_(1e9)
+        ops.paged_attention(gpu, a)
+        torch.cuda.synchronize()
+        assert torch.all(space[:64] == 1e9) and torch.all(space[64 + n // 4:] == 1e9)
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
 def test_pages_beyond_32_bits(gpu, kind):
     """Pages 3 GiB apart, 9 GiB from the first to the last."""
     cache = Cache([64], "f16", kind, 1, 64, 16)
@@ -484,11 +523,11 @@ def test_documents_that_share_pages(gpu, kind):
     assert_within(t.out, out, out_tol, "out")
 
 
-@pytest.mark.parametrize("documents", [70, 3000])
-def test_many_documents(gpu, documents):
-    lengths = [1 + i % 40 for i in range(documents)]
+@pytest.mark.parametrize("documents,queries", [(64, 1), (65, 1), (70, 30), (3000, 1)])
+def test_many_documents(gpu, documents, queries):
+    lengths = [queries + i % 40 for i in range(documents)]
     cache = Cache(lengths, "f16", "plain", 1, 64, 16, fill=True)
-    t = Queries(cache, [1] * documents, "f16", 2)
+    t = Queries(cache, [queries if i % 3 else 1 for i in range(documents)], "f16", 2)
     ops.paged_attention(gpu, t.args(gpu))
     out, out_tol, _, _ = t.reference()
     assert_within(t.out, out, out_tol, "out")
