@@ -660,3 +660,43 @@ def test_no_rows_and_no_pages(gpu, kind):
     c.cache.pages, c.cache.k.data, c.cache.v.data = 0, None, None
     ops.cache_append(gpu, b.table, c)  # the queries are turned all the same
     assert not bool((b.q_out == SENTINEL).all())
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("queries", [2, 90])
+def test_one_document_without_offsets(gpu, kind, queries):
+    cache = Cache([700], "bf16", kind, 2, 64, 32)
+    t = Queries(cache, [queries], "bf16", 4)
+    a = t.args(gpu)
+    a.q_offsets = None
+    ops.paged_attention(gpu, a)
+    out, out_tol, lse, lse_tol = t.reference()
+    assert_within(t.out, out, out_tol, "out")
+    assert_within(t.lse, lse, lse_tol, "lse")
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+def test_keys_and_values_side_by_side_among_layers(gpu, kind):
+    """One allocation holds two layers' pages, each row's key and value beside each
+    other: append, attention and read go by strides, and touch their own layer alone."""
+    d, page, kv, pages = 64, 16, 2, 6
+    row = 40 if kind == "int4" else 128
+    arena = torch.full((pages, 2, page, kv, 2, row), 0xFF, device="cuda", dtype=torch.uint8)
+    cache = Cache([50, 20], "f16", kind, kv, d, page, max_pages=4)
+    cache.pages, cache.table_list = pages, [[5, 1, 2, 0], [3, 4, -1, -1]]
+    cache.table.copy_(torch.tensor(cache.table_list))
+    cache.pools = [arena[:, 1, :, :, side] for side in range(2)]
+    t = Append(cache, [50, 20], "f16", 4, [32])
+    other = arena[:, 0].clone()
+    before = [p.clone() for p in cache.pools]
+    ops.cache_append(gpu, t.table, t.args())
+    t.check(before)
+    assert torch.equal(arena[:, 0], other)
+    back = [torch.zeros(70, kv, d, device="cuda", dtype=torch.float16) for _ in range(2)]
+    ops.cache_read(gpu, ops.CacheReadArgs(dtype=hip.F16, rows=70, documents=2, kv_heads=kv, head_dim=d, offsets=at(t.offsets), k_out=heads(back[0]),
+                                          v_out=heads(back[1]), cache=cache.struct()))
+    cache.rows = [[b[:50].double(), b[50:].double()] for b in back]
+    q = Queries(cache, [3, 20], "f16", 4)
+    ops.paged_attention(gpu, q.args(gpu))
+    out, out_tol, _, _ = q.reference()
+    assert_within(q.out, out, out_tol, "out")
