@@ -74,8 +74,8 @@ bl::HeadsParams heads_params(const bl_rotary_table *t, const bl_head_norm_args *
     bl::HeadsParams p{};
     if (t) p.table = *t;
     p.positions = a->positions;
-    p.q_gamma = a->q_gamma;
-    p.k_gamma = a->k_gamma;
+    p.q_gamma = a->q_heads ? a->q_gamma : nullptr;  // weights of no heads are not looked at, and may be any address
+    p.k_gamma = a->k_heads ? a->k_gamma : nullptr;
     p.q_in = a->q_in;
     p.q_out = a->q_out;
     p.k_in = a->k_in;
