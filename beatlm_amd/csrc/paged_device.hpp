@@ -23,16 +23,19 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 struct PagedDocument {
     int q0, n_q;
-    int n_k, shift;  // query i stands at key i + shift
+    int n_k;    // keys that the table's row has room for
+    int shift;  // query i stands at key i + shift, by the whole length, as it was appended
     int index;
 };
 
-// A document's first row, rows and keys, whatever the arrays hold; any lane's own.
-__device__ __forceinline__ void bounds_of(const bl_paged_attention_args &a, int d, int &q0, int &n_q, int &n_k) {
+// A document's first row, rows, length and keys, whatever the arrays hold; any
+// lane's own.
+__device__ __forceinline__ void bounds_of(const bl_paged_attention_args &a, int d, int &q0, int &n_q, int &length, int &n_k) {
     const int rows = (int)a.q_rows;
     q0 = a.q_offsets ? min(max(a.q_offsets[d], 0), rows) : 0;
     n_q = max((a.q_offsets ? min(max(a.q_offsets[d + 1], 0), rows) : rows) - q0, 0);
-    n_k = min(max(a.cache.lengths[d], 0), (int)(a.cache.max_pages * a.cache.page_rows));
+    length = max(a.cache.lengths[d], 0);
+    n_k = min(length, (int)(a.cache.max_pages * a.cache.page_rows));
 }
 
 // Which document and which of its tiles of `tile` places a workgroup has; tile
@@ -46,8 +49,8 @@ struct Assignment {
         const int documents = (int)a.documents;
         if (documents <= 64) {
             const int lane = threadIdx.x % 64;
-            int q0, n_q, n_k;
-            bounds_of(a, min(lane, documents - 1), q0, n_q, n_k);
+            int q0, n_q, length, n_k;
+            bounds_of(a, min(lane, documents - 1), q0, n_q, length, n_k);
             const int tiles = lane < documents ? (int)(((int64_t)n_q * group + tile_places - 1) / tile_places) : 0;
             const int cost = a.window ? (int)min((int64_t)n_k, (int64_t)n_q + a.window) : n_k;
             int first = 0;  // tiles of the documents that go before the lane's
@@ -61,27 +64,29 @@ struct Assignment {
             doc.q0 = __builtin_amdgcn_readlane(q0, at);
             doc.n_q = __builtin_amdgcn_readlane(n_q, at);
             doc.n_k = __builtin_amdgcn_readlane(n_k, at);
+            doc.shift = __builtin_amdgcn_readlane(length - n_q, at);
             // A causal document's last places see the most keys.
             tile = found ? __builtin_amdgcn_readlane(tiles, at) - 1 - (slot - __builtin_amdgcn_readlane(first, at)) : -1;
         } else {
             const int back = (int)slots(a.q_rows, group, tile_places, documents) - 1 - slot;
             doc.index = document_of_slot(a.q_offsets, documents, a.q_rows, group, tile_places, back);
-            bounds_of(a, doc.index, doc.q0, doc.n_q, doc.n_k);
+            int length;
+            bounds_of(a, doc.index, doc.q0, doc.n_q, length, doc.n_k);
             doc.q0 = uniform(doc.q0);
             doc.n_q = uniform(doc.n_q);
             doc.n_k = uniform(doc.n_k);
+            doc.shift = uniform(length) - doc.n_q;
             tile = back - ((int)((int64_t)doc.q0 * group / tile_places) + doc.index);
             if ((int64_t)tile * tile_places >= (int64_t)doc.n_q * group) tile = -1;
         }
-        doc.shift = doc.n_k - doc.n_q;
     }
 };
-// Query i sees keys [from, to).
+// Query i sees keys [from, to), both within the keys that there are.
 __device__ __forceinline__ int keys_to(const bl_paged_attention_args &a, const PagedDocument &doc, int i) {
     return a.mask == BL_MASK_NONE ? doc.n_k : min(doc.n_k, max(i + doc.shift + 1, 0));
 }
 __device__ __forceinline__ int keys_from(const bl_paged_attention_args &a, const PagedDocument &doc, int i) {
-    return a.window ? (int)max((int64_t)0, (int64_t)i + doc.shift + 1 - (int64_t)a.window) : 0;
+    return a.window ? (int)min((int64_t)doc.n_k, max((int64_t)0, (int64_t)i + doc.shift + 1 - (int64_t)a.window)) : 0;
 }
 
 // A workgroup's share of the tiles that its places see: equal ones, so that a

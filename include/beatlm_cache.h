@@ -82,8 +82,9 @@ int bl_head_norm_rotary_backward(bl_ctx *ctx, const bl_rotary_table *table, cons
  *
  * table and lengths are device arrays, read when the kernels run. A page
  * number outside the cache is a page that is not there (one given back, or
- * never dealt out): nothing is written to it and its keys are not seen. Lengths
- * are clamped to the table's row. Pages may be shared by documents that read
+ * never dealt out): nothing is written to it and its keys are not seen; neither
+ * are keys beyond the table's row, of a longer document, whose places count from
+ * its whole length all the same. Pages may be shared by documents that read
  * them.
  * ------------------------------------------------------------------------ */
 enum { BL_CACHE_PLAIN = 0, BL_CACHE_INT4 = 1 };
