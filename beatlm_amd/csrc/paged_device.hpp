@@ -217,4 +217,11 @@ template <int N> __device__ __forceinline__ void values_of(uint32_t w, f16x2 ste
 
 __device__ __forceinline__ f16x2 both(uint32_t bits) { return __builtin_bit_cast(f16x2, bits); }
 
+// Whether some code of a group stands for an infinity or NaN: the last one does
+// then, as what codes stand for rises or falls from low to it.
+__device__ __forceinline__ bool infinite_codes(uint32_t params) {
+    const f16x2 p = both(params);
+    return !(__builtin_fabsf16(__builtin_fmaf16((_Float16)15.0f, p[0], p[1])) < (_Float16)INFINITY);
+}
+
 }  // namespace bl
