@@ -16,6 +16,19 @@ Named heads_named(const bl_heads &h, uint64_t rows, uint64_t heads, uint64_t hea
     return {bytes_of(h, rows, heads, head_dim, size), name};
 }
 Named weights_named(const void *p, uint64_t head_dim, uint64_t size, const char *name) { return {bytes_of({(void *)p, 0, 0}, 1, 1, head_dim, size), name}; }
+// Bytes next to each other: indices, weights' gradients, a workspace.
+Named block_named(const void *p, uint64_t bytes, const char *name) { return {{(uint64_t)p, 0, 1, 0, p && bytes ? 1u : 0u, bytes}, name}; }
+Named positions_named(const bl_rotary_table *t, const int32_t *positions, uint64_t rows) {
+    return block_named(t ? positions : nullptr, t ? rows * t->axes * 4 : 0, "positions");
+}
+// A call's outputs beside indices that it reads.
+template <size_t N, size_t M>
+int check_outputs_apart(bl_ctx *ctx, const char *what, const Named (&written)[N], const Named (&read)[M]) {
+    for (const Named &out : written)
+        for (const Named &in : read)
+            if (int rc = check_apart(ctx, what, out, in)) return rc;
+    return BL_OK;
+}
 
 // ---- norms of heads ----
 
@@ -142,6 +155,23 @@ Steps steps_of(const bl_paged_cache &c, const bl_pages &p, uint32_t heads) {
     s.add(p.head_stride, heads);
     return s;
 }
+// Whether a block of bytes meets a row of one of the n smallest steps, the first
+// row at 0; steps sorted, rows apart. A step's copies that the block meets are
+// neighbours, and of three the middle one lies in it whole.
+bool meets(const Steps &s, int n, wide from, wide to, uint64_t width) {
+    if (n == 0) return from < (wide)width && to > 0;
+    wide extent = width;
+    for (int i = 0; i < n - 1; i++) extent += (wide)s.step[i] * (s.count[i] - 1);
+    const wide step = s.step[n - 1];
+    if (to <= 0) return false;
+    const wide first = from < extent ? 0 : (from - extent) / step + 1, end = (to - 1) / step + 1;
+    const wide last = (end < (wide)s.count[n - 1] ? end : (wide)s.count[n - 1]) - 1;
+    if (last - first >= 2) return true;
+    for (wide i = first; i <= last; i++)
+        if (meets(s, n - 1, from - i * step, to - i * step, width)) return true;
+    return false;
+}
+
 // All the bytes of a side from its first to its last.
 Bytes extent_of(const bl_paged_cache &c, const bl_pages &p, uint32_t heads, uint64_t width) {
     const uint64_t last = c.pages ? (c.pages - 1) * p.page_stride + (c.page_rows - 1) * p.row_stride + (heads - 1) * p.head_stride + width : 0;
@@ -179,6 +209,25 @@ int check_cache(bl_ctx *ctx, const bl_paged_cache &c, uint32_t dtype, uint32_t h
     }
     return BL_OK;
 }
+
+// Blocks beside the pages of both sides: the gaps between pages' rows are anyone's.
+template <size_t N>
+int check_blocks_beside_pages(bl_ctx *ctx, const bl_paged_cache &c, uint32_t heads, uint64_t width, const Named (&blocks)[N], const char *what) {
+    if (c.pages == 0) return BL_OK;
+    const bl_pages *const sides[] = {&c.k, &c.v};
+    for (const Named &block : blocks)
+        for (int n = 0; n < 2; n++) {
+            if (block.bytes.rows == 0 || !overlap(block.bytes, extent_of(c, *sides[n], heads, width))) continue;
+            Steps s = steps_of(c, *sides[n], heads);
+            const wide from = (wide)block.bytes.at - (wide)(uint64_t)sides[n]->data;
+            if (!s.apart(width) || meets(s, s.n, from, from + (wide)block.bytes.width, width))
+                return refuse(ctx, BL_ERR_INVALID_ARGUMENT, "%s: %s overlaps the cache's %s", what, block.name, n == 0 ? "keys" : "values");
+        }
+    return BL_OK;
+}
+Named table_named(const bl_paged_cache &c, uint64_t documents) { return block_named(c.table, documents * c.max_pages * 4, "the cache's table"); }
+Named lengths_named(const bl_paged_cache &c, uint64_t documents) { return block_named(c.lengths, documents * 4, "the cache's lengths"); }
+Named offsets_named(const int32_t *offsets, uint64_t documents, const char *name) { return block_named(offsets, (documents + 1) * 4, name); }
 
 int check_documents(bl_ctx *ctx, uint32_t documents, const int32_t *offsets, const char *what) {
     if (documents == 0) return refuse(ctx, BL_ERR_INVALID_ARGUMENT, "%s: no documents", what);
@@ -240,6 +289,7 @@ extern "C" int bl_head_norm_rotary(bl_ctx *ctx, const bl_rotary_table *t, const 
         for (const Named &w : {weights_named(a->q_heads ? a->q_gamma : nullptr, a->head_dim, size, "q_gamma"), weights_named(a->k_heads ? a->k_gamma : nullptr, a->head_dim, size, "k_gamma")})
             if (w.bytes.at)
                 if (int rc = check_apart(ctx, what, out, w)) return rc;
+    if (int rc = check_outputs_apart(ctx, what, {q_out, k_out}, {positions_named(t, a->positions, a->rows)})) return rc;
     if (a->rows == 0) return BL_OK;
     bl::HeadsParams p = heads_params(t, a);
     Widest w(a->dtype);
@@ -306,6 +356,10 @@ extern "C" int bl_head_norm_rotary_backward(bl_ctx *ctx, const bl_rotary_table *
                       (unsigned long long)need);
     if (!g->workspace || !aligned(g->workspace, 16))
         return refuse(ctx, BL_ERR_MISALIGNED_PLACEMENT, "%s: the workspace is null or not 16-byte aligned", what);
+    if (int rc = check_outputs_apart(ctx, what, {dq_in, dk_in}, {positions_named(t, a->positions, a->rows)})) return rc;
+    const Named floats[] = {block_named(a->q_heads ? g->d_q_gamma : nullptr, a->head_dim * 4, "d_q_gamma"),
+                            block_named(a->k_heads ? g->d_k_gamma : nullptr, a->head_dim * 4, "d_k_gamma"), block_named(g->workspace, need, "the workspace")};
+    if (int rc = check_outputs_apart(ctx, what, floats, {q_in, dq_out, dq_in, k_in, dk_out, dk_in})) return rc;
     bl::HeadsParams p = heads_params(t, a);
     p.dq_out = g->dq_out;
     p.dk_out = g->dk_out;
@@ -371,6 +425,13 @@ extern "C" int bl_cache_append(bl_ctx *ctx, const bl_rotary_table *t, const bl_c
     for (const Named &w : {weights_named(q_gamma, a->head_dim, size, "q_gamma"), weights_named(k_gamma, a->head_dim, size, "k_gamma")})
         if (w.bytes.at)
             if (int rc = check_apart(ctx, what, q_out, w)) return rc;
+    const Named indices[] = {positions_named(t, a->positions, a->rows), offsets_named(a->q_offsets, a->documents, "q_offsets"),
+                             table_named(a->cache, a->documents), lengths_named(a->cache, a->documents)};
+    if (int rc = check_outputs_apart(ctx, what, {q_out}, indices)) return rc;
+    if (int rc = check_blocks_beside_pages(ctx, a->cache, a->kv_heads, width, indices, what)) return rc;
+    if (int rc = check_blocks_beside_pages(ctx, a->cache, a->kv_heads, width,
+                                           {block_named(q_gamma, a->head_dim * size, "q_gamma"), block_named(k_gamma, a->head_dim * size, "k_gamma")}, what))
+        return rc;
     if (a->rows == 0) return BL_OK;
     bl::AppendParams p{};
     if (t) p.h.table = *t;
@@ -426,6 +487,9 @@ extern "C" int bl_cache_read(bl_ctx *ctx, const bl_cache_read_args *a) {
         for (const Named &side : {Named{extent_of(a->cache, a->cache.k, a->kv_heads, width), "the cache's keys"},
                                   Named{extent_of(a->cache, a->cache.v, a->kv_heads, width), "the cache's values"}})
             if (int rc = check_apart(ctx, what, out, side)) return rc;
+    if (int rc = check_outputs_apart(ctx, what, {k_out, v_out}, {offsets_named(a->offsets, a->documents, "offsets"), block_named(a->first, a->documents * 4ull, "first"),
+                                                                table_named(a->cache, a->documents), lengths_named(a->cache, a->documents)}))
+        return rc;
     if (a->rows == 0) return BL_OK;
     const DeviceScope scope(bl_device_of(ctx));
     if (scope.status != hipSuccess) return launched(ctx, scope.status, what);
@@ -454,7 +518,8 @@ extern "C" int bl_paged_attention(bl_ctx *ctx, const bl_paged_attention_args *a)
     if (int rc = check_cache(ctx, a->cache, a->dtype, a->kv_heads, a->head_dim, false, what)) return rc;
     const uint64_t size = element_size(a->dtype), width = row_bytes(a->cache, a->dtype, a->head_dim);
     const Named out = heads_named(a->out, a->q_rows, a->q_heads, a->head_dim, size, "out");
-    for (const Named &other : {heads_named(a->q, a->q_rows, a->q_heads, a->head_dim, size, "q"), Named{extent_of(a->cache, a->cache.k, a->kv_heads, width), "the cache's keys"},
+    const Named q = heads_named(a->q, a->q_rows, a->q_heads, a->head_dim, size, "q");
+    for (const Named &other : {q, Named{extent_of(a->cache, a->cache.k, a->kv_heads, width), "the cache's keys"},
                                Named{extent_of(a->cache, a->cache.v, a->kv_heads, width), "the cache's values"}})
         if (int rc = check_apart(ctx, what, out, other)) return rc;
     const bl::PagedPlan plan = bl::plan_paged(*a, bl_compute_units_of(ctx));
@@ -464,6 +529,12 @@ extern "C" int bl_paged_attention(bl_ctx *ctx, const bl_paged_attention_args *a)
                       (unsigned long long)need);
     if (need && (!a->workspace || !aligned(a->workspace, 16)))
         return refuse(ctx, BL_ERR_MISALIGNED_PLACEMENT, "%s: the workspace is null or not 16-byte aligned", what);
+    if (int rc = check_outputs_apart(ctx, what, {out}, {offsets_named(a->q_offsets, a->documents, "q_offsets"), table_named(a->cache, a->documents),
+                                                       lengths_named(a->cache, a->documents)}))
+        return rc;
+    const Named floats[] = {block_named(a->lse, (uint64_t)a->q_rows * a->q_heads * 4, "lse"), block_named(a->workspace, need, "the workspace")};
+    if (int rc = check_outputs_apart(ctx, what, floats, {q, out})) return rc;
+    if (int rc = check_blocks_beside_pages(ctx, a->cache, a->kv_heads, width, floats, what)) return rc;
     if (a->q_rows == 0) return BL_OK;
     const DeviceScope scope(bl_device_of(ctx));
     if (scope.status != hipSuccess) return launched(ctx, scope.status, what);

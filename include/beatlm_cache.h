@@ -11,6 +11,13 @@
  * nothing allocated and nothing waited for, argument structs read during the
  * call alone and device arrays when the kernels run, a workspace for each call
  * that may overlap another, and a refused call launches nothing.
+ *
+ * Tensors and pages that a call writes share no byte with what else it reads or
+ * writes, other than where an output may be an input itself, and lse, weights'
+ * gradients and a workspace none with tensors and pages: such a call is refused.
+ * Not looked at, and the host's to keep apart: lse, gradients and workspace
+ * beside each other and beside weights and index arrays, and what the device
+ * arrays say (two rows of a call for one row of a page).
  */
 #ifndef BEATLM_CACHE_H
 #define BEATLM_CACHE_H
