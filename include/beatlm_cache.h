@@ -122,7 +122,9 @@ typedef struct {
  * (n > lengths[d]), beyond the table or of a page that is not there is dropped;
  * its query is turned all the same. Rows of no document are not touched, and
  * of the cache nothing but the new keys' rows. A page's row that two rows of a
- * call are appended to holds one of the two.
+ * call are appended to (a page in two documents' tables) may hold parts of both,
+ * codes of one under a step and low of the other: a shared page is copied before
+ * a document goes on in it.
  *
  * q_out and PLAIN keys are computed in f32 and rounded once; values are copied.
  * INT4: low is the smallest value of a group, step (largest - smallest) / 15,
