@@ -132,7 +132,9 @@ typedef struct {
  * - low) / step (ties to even, 0 to 15). Keys are computed in 64 bits for it and
  * rounded to f32, and codes are found in 64 bits, so a key gets the same codes
  * in a chunk as alone. A group that holds a NaN or a magnitude above 65504
- * stands for NaN. */
+ * stands for NaN. Values up to 65440 in magnitude stand for finite ones: low and
+ * step are off by at most 16 and 4, and 65440 + 16 + 15 * 4 is under 65520, where
+ * f16 rounds to infinity. With larger ones a group's last code may stand for it. */
 typedef struct {
     uint32_t dtype;             /* of q, k, v and a PLAIN cache */
     uint32_t rows;              /* of q, k and v */
