@@ -294,6 +294,24 @@ __device__ __forceinline__ void store_partial(float *at, int half, const f32x16 
 // is from |x| = 1 on. With a cap, s = cap tanh(u), u = scale qk / cap. `factor` is
 // what x is of a product, or of its tanh.
 
+// tanh(u) for |u| < TANH_NEAR: a polynomial in u^2 (fitted to tanh(u) / u at
+// Chebyshev points) that is off by less than a step of f32.
+template <bool F32> constexpr float TANH_NEAR = F32 ? 1.0f : 0.5f;
+template <bool F32> __device__ __forceinline__ float tanh_near_zero(float u) {
+    const float w = u * u;
+    float v;
+    if constexpr (F32) {
+        v = 0.00228764559f + w * -0.000354883407f;
+        v = 0.0214699805f + w * (-0.00792494603f + w * v);
+        v = 0.133321911f + w * (-0.053872738f + w * v);
+        v = 1.0f + w * (-0.333332807f + w * v);
+    } else {
+        v = 0.133248284f + w * (-0.0529892407f + w * 0.0171413198f);
+        v = 1.0f + w * (-0.333330721f + w * v);
+    }
+    return u * v;
+}
+
 template <typename T, bool CAP> struct Scores {
     float factor;  // log2(e) scale, or log2(e) cap
     float inner;   // scale / cap
@@ -307,35 +325,21 @@ template <typename T, bool CAP> struct Scores {
         inner = CAP ? scale / a.softcap : 0.0f;
     }
     // With a cap, products to their tanh u. Where a wave's tile has no |u| of
-    // LIMIT or more, the usual case as caps are wide, a polynomial in u^2
-    // (fitted to tanh(u) / u at Chebyshev points) that is off by less than a
-    // step of f32: 4 or 7 multiplications more than the product itself, 28
-    // cycles a wave for the 16-bit types. Any other tile: 1 - 2 / (e^2u + 1),
-    // off by a few steps of 1, 44 cycles with its two quarter-rate
-    // instructions; f32 takes tanhf, some ten times that.
+    // LIMIT or more, the usual case as caps are wide, the polynomial: 4 or 7
+    // multiplications more than the product itself, 28 cycles a wave for the
+    // 16-bit types. Any other tile: 1 - 2 / (e^2u + 1), off by a few steps of
+    // 1, 44 cycles with its two quarter-rate instructions; f32 takes tanhf, some
+    // ten times that.
     __device__ __forceinline__ void caps(f32x16 &s) const {
         if constexpr (!CAP) return;
         constexpr bool F32 = sizeof(T) == 4;
-        constexpr float LIMIT = F32 ? 1.0f : 0.5f;
+        constexpr float LIMIT = TANH_NEAR<F32>;
         float top = 0.0f;
 #pragma unroll
         for (int r = 0; r < 16; r += 2) top = fmaxf(fmaxf(fabsf(s[r]), fabsf(s[r + 1])), top);
         if (__all(top * fabsf(inner) < LIMIT)) {  // a NaN is no maximum, and stays one in either form
 #pragma unroll
-            for (int r = 0; r < 16; r++) {
-                const float u = s[r] * inner, w = u * u;
-                float v;
-                if constexpr (F32) {
-                    v = 0.00228764559f + w * -0.000354883407f;
-                    v = 0.0214699805f + w * (-0.00792494603f + w * v);
-                    v = 0.133321911f + w * (-0.053872738f + w * v);
-                    v = 1.0f + w * (-0.333332807f + w * v);
-                } else {
-                    v = 0.133248284f + w * (-0.0529892407f + w * 0.0171413198f);
-                    v = 1.0f + w * (-0.333330721f + w * v);
-                }
-                s[r] = u * v;
-            }
+            for (int r = 0; r < 16; r++) s[r] = tanh_near_zero<F32>(s[r] * inner);
         } else if constexpr (F32) {
 #pragma unroll
             for (int r = 0; r < 16; r++) s[r] = tanhf(s[r] * inner);
