@@ -12,7 +12,7 @@
 // step's few tokens, beside which the first heads are on their way: 32 tokens of
 // 16 + 4 heads of 128, bf16, 6.6 us. 8192 tokens of them into 4-bit pages 27 us,
 // 3.3 TB/s: the keys' 64 bits leave a SIMD three or four waves, whose vector
-// instructions are some 60 % of the cycles (codes found in 64 bits throughout,
+// instructions are half of the cycles (codes found in 64 bits throughout,
 // sines in LDS as large as any call needs and two heads a row at once: 35).
 #include "heads_device.hpp"
 

@@ -16,6 +16,13 @@ hipError_t run_kernel(void (*kernel)(P...), dim3 grid, uint32_t threads, hipStre
     return hipLaunchKernel((const void *)kernel, grid, dim3(threads), args, 0, s);
 }
 
+// The same with `lds` bytes of LDS beside what the kernel declares.
+template <typename... P>
+hipError_t run_kernel_with(uint32_t lds, void (*kernel)(P...), dim3 grid, uint32_t threads, hipStream_t s, const P &...params) {
+    void *args[] = {(void *)&params...};
+    return hipLaunchKernel((const void *)kernel, grid, dim3(threads), args, lds, s);
+}
+
 // Lane l and lane l ^ 16, as max_xor32 and sum_xor32: the swap exchanges the odd
 // rows of 16 lanes of its first operand with the even ones of its second.
 __device__ __forceinline__ float max_xor16(float v) {
@@ -25,13 +32,6 @@ __device__ __forceinline__ float max_xor16(float v) {
 __device__ __forceinline__ float sum_xor16(float v) {
     const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-
-// The same with `lds` bytes of LDS beside what the kernel declares.
-template <typename... P>
-hipError_t run_kernel_with(uint32_t lds, void (*kernel)(P...), dim3 grid, uint32_t threads, hipStream_t s, const P &...params) {
-    void *args[] = {(void *)&params...};
-    return hipLaunchKernel((const void *)kernel, grid, dim3(threads), args, lds, s);
 }
 
 // VEC elements at p (16-byte aligned when VEC > 1) as f32.

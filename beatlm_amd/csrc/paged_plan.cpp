@@ -41,9 +41,10 @@ PagedPlan plan_paged(const bl_paged_attention_args &a, uint32_t compute_units) {
         plan.splits = (uint32_t)((keys + plan.share - 1) / plan.share);
     } else {
         // Even shares of each document: four workgroups a compute unit (16 tokens over
-        // 3449 to 16326 keys, 4 key heads of 128, bf16: 67 us; in two 72, in eight 73.
-        // 32 over 3300 to 16153 in codes, 8 key heads: 102; in three 97, in eight 100;
-        // heads of 64 58, 66 and 64).
+        // 3449 to 16326 keys, 4 key heads of 128, bf16: 72 us; in two 74, three 72, eight
+        // 73; heads of 64 34, 38, 36 and 37. 32 over 3300 to 16153 in codes, 8 key heads
+        // of 64: 57; 73, 60 and 62). Heads of 128 in codes are the exception, as a
+        // compute unit holds three of their workgroups: 109, and 116, 96 and 104.
         const uint64_t wanted = whole < 4 * units ? (4 * units + whole - 1) / whole : 1, most = (keys + 127) / 128;
         plan.splits = (uint32_t)(wanted < most ? wanted : most);
         // Few keys: eight waves a workgroup, one or two steps each, and no second launch

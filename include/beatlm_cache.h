@@ -130,8 +130,8 @@ typedef struct {
  * INT4: low is the smallest value of a group, step (largest - smallest) / 15,
  * each rounded to f32 and then to f16, and a code the nearest integer to (value
  * - low) / step (ties to even, 0 to 15). Keys are computed in 64 bits for it and
- * rounded to f32, and codes are found in 64 bits, so a key gets the same codes
- * in a chunk as alone. A group that holds a NaN or a magnitude above 65504
+ * rounded to f32, and codes are those of 64 bits: the definition's, whatever
+ * alignment the call's tensors have. A group that holds a NaN or a magnitude above 65504
  * stands for NaN. Values up to 65440 in magnitude stand for finite ones: low and
  * step are off by at most 16 and 4, and 65440 + 16 + 15 * 4 is under 65520, where
  * f16 rounds to infinity. With larger ones a group's last code may stand for it. */
@@ -179,11 +179,13 @@ int bl_cache_read(bl_ctx *ctx, const bl_cache_read_args *args);
  *
  * A row that sees no key gets out = 0 and lse = -inf; rows of no document are
  * not touched. Rows of a page beyond the document's length are never read, and
- * hidden keys, and pages that are not there, may hold anything. Statistics, sums and scores are f32. For the
- * matrix cores probabilities are rounded to the tensors' type over a PLAIN
- * cache and to f16 over INT4, where queries are taken times a power of two of
- * each row that keeps them in f16's range; f32 over INT4 takes queries and
- * probabilities as two f16 each. No atomics: equal calls give equal bits. */
+ * hidden keys, and pages that are not there, may hold anything. A NaN key makes
+ * NaN of the rows that see it, infinite and NaN values of their channels (f32
+ * over INT4: an infinite key may do as a NaN). Statistics, sums and scores are
+ * f32. For the matrix cores probabilities are rounded to the tensors' type over
+ * a PLAIN cache and to f16 over INT4, where queries are taken times a power of
+ * two of each row that keeps them in f16's range; f32 over INT4 takes queries
+ * and probabilities as two f16 each. No atomics: equal calls give equal bits. */
 typedef struct {
     uint32_t dtype;             /* of q, out and a PLAIN cache */
     uint32_t q_heads, kv_heads; /* q_heads a multiple of kv_heads */
