@@ -183,9 +183,10 @@ int bl_cache_read(bl_ctx *ctx, const bl_cache_read_args *args);
  * NaN of the rows that see it, infinite and NaN values of their channels (f32
  * over INT4: an infinite key may do as a NaN). Statistics, sums and scores are
  * f32. For the matrix cores probabilities are rounded to the tensors' type over
- * a PLAIN cache and to f16 over INT4, where queries are taken times a power of
- * two of each row that keeps them in f16's range; f32 over INT4 takes queries
- * and probabilities as two f16 each. No atomics: equal calls give equal bits. */
+ * a PLAIN cache (bf16 of few queries a document keeps 15 bits) and to f16 over
+ * INT4, where queries are taken times a power of two of each row that keeps them
+ * in f16's range; f32 over INT4 takes queries and probabilities as two f16 each.
+ * No atomics: equal calls give equal bits. */
 typedef struct {
     uint32_t dtype;             /* of q, out and a PLAIN cache */
     uint32_t q_heads, kv_heads; /* q_heads a multiple of kv_heads */
